@@ -173,6 +173,90 @@ int f2s_neighbor_reduce_tc(const float* content, const float* geometry, const in
 int f2s_linear(const void* x, int ldx, const void* weight, const float* bias, float* y, int ldy,
                int rows, int cols, int K, int precision, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* A feed-forward layer in 8 bits (no counterpart in the reference, whose     */
+/* trunk runs in fp32): RMS norm, 8-bit rows and their product, SwiGLU        */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the activations of this section. */
+typedef enum f2s_dtype { F2S_DTYPE_F32 = 0, F2S_DTYPE_BF16 = 1, F2S_DTYPE_F16 = 2 } f2s_dtype;
+
+/*
+ * Rows: (rows, C) matrices of `dtype` whose rows start ld elements apart
+ * (ld >= C). Any alignment and pitch is taken; bases and pitches of whole
+ * 16-byte vectors (and C a multiple of the vector) are read and written 16
+ * bytes at a time. C at most 32768 where a kernel holds a row in registers
+ * (F2S_ERR_UNSUPPORTED beyond). All arithmetic is fp32.
+ *
+ * 8-bit rows: q (rows, C) int8 of pitch ldq and one fp32 scale per row, standing
+ * for scale * q. q is the whole number nearest to 127 v / max|v| (of the exact
+ * quotient, the even one at a tie), scale = max|v| / 127. A row of zeros has
+ * scale 0; a row with a value that is not finite has q 0 and scale NaN.
+ *
+ * Root-mean-square norm of a residual stream:
+ *   s = x + residual, rounded to dtype and written to stream_out (rows, C);
+ *   y = s (mean(s^2) + eps)^-1/2 weight.
+ * residual NULL: s = x and stream_out is not touched. weight (C) of dtype.
+ * y (rows, C), or 8-bit rows of it (q, scale).
+ */
+int f2s_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                     const void* weight, int dtype, int64_t rows, int C, float eps,
+                     void* stream_out, void* y, void* stream);
+int f2s_add_rms_norm_int8(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                          const void* weight, int dtype, int64_t rows, int C, float eps,
+                          void* stream_out, int8_t* q, int64_t ldq, float* scale, void* stream);
+
+/*
+ * Backward of f2s_add_rms_norm from the stream s: dx (rows, C) is the gradient
+ * of x and of the residual alike, given dy and (or NULL) the gradient ds of the
+ * stream output; dweight (C) of dtype, or NULL. The sums over rows are fp32 in
+ * a fixed order.
+ *   workspace (dweight only): f2s_add_rms_norm_backward_workspace_bytes().
+ */
+int f2s_add_rms_norm_backward_workspace_bytes(int64_t rows, int C, size_t* bytes);
+int f2s_add_rms_norm_backward(const void* s, int64_t lds, const void* weight, int dtype,
+                              int64_t rows, int C, float eps, const void* dy, int64_t lddy,
+                              const void* ds, int64_t ldds, void* dx, void* dweight,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows to 8 bits, and back to dtype. */
+int f2s_quantize_rows(const void* x, int64_t ldx, int dtype, int64_t rows, int C, int8_t* q,
+                      int64_t ldq, float* scale, void* stream);
+int f2s_dequantize_rows(const int8_t* q, int64_t ldq, const float* scale, int64_t rows, int C,
+                        void* y, int64_t ldy, int dtype, void* stream);
+
+/*
+ * y[t, n] = x_scale[t] w_scale[n] sum_k x[t, k] w[n, k] + bias[n]: x (rows, K)
+ * and w (cols, K) 8-bit rows, the sum exact in 32 bits (K <= 131071,
+ * F2S_ERR_UNSUPPORTED beyond); bias (cols) of dtype or NULL; y of dtype and
+ * pitch ldy. On tcgen05 where x and w start on 16 bytes with pitches that are
+ * multiples of 16 (as f2s_quantize_rows can lay them out); other pitches run
+ * on the CUDA cores.
+ */
+int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                    int64_t ldw, const float* w_scale, const void* bias, void* y, int64_t ldy,
+                    int dtype, int rows, int cols, int K, void* stream);
+
+/*
+ * SwiGLU of a packed projection (rows, 2 H) = [gate | value]:
+ * y = value gate sigma(gate), (rows, H).
+ * checkpoint / checkpoint_scale (both or neither): the gate and value rows kept
+ * in 8 bits for the backward. With G = ceil(H / F2S_SWIGLU_GROUP) groups of
+ * channels a row takes G * 2 * F2S_SWIGLU_GROUP bytes and 2 G scales (gate and
+ * value of each group, its channels in an order that depends on H alone).
+ * The backward gives dprojected (rows, 2 H) from the checkpoint, or, where that
+ * is NULL, from the projection itself.
+ * f2s_swiglu_int8: y as 8-bit rows.
+ */
+#define F2S_SWIGLU_GROUP 128
+int f2s_swiglu(const void* projected, int64_t ld, int dtype, int64_t rows, int H, void* y,
+               int8_t* checkpoint, float* checkpoint_scale, void* stream);
+int f2s_swiglu_backward(const void* projected, int64_t ld, const int8_t* checkpoint,
+                        const float* checkpoint_scale, const void* dy, int64_t lddy, int dtype,
+                        int64_t rows, int H, void* dprojected, void* stream);
+int f2s_swiglu_int8(const void* projected, int64_t ld, int dtype, int64_t rows, int H, int8_t* q,
+                    int64_t ldq, float* scale, void* stream);
+
 /*
  * The library's device error word: 1 when a tensor-core kernel gave up on a
  * bounded wait (it then returned without finishing its tile), 2 when an fp16

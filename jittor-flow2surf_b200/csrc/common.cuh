@@ -48,6 +48,10 @@ enum TraceTag {
     kTagNearest,
     kTagTranspose,
     kTagTraining,
+    kTagRmsNorm,
+    kTagRows8,
+    kTagSwiGlu,
+    kTagGemmInt8,
     kTagCount
 };
 

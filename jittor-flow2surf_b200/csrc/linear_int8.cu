@@ -1,0 +1,99 @@
+// Product of 8-bit integer rows with scales for each token and channel:
+//   y[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k] + b[n],
+// the sum exact in 32 bits (K <= 131,071 keeps 2^14 K below 2^31).
+#include "kernels.cuh"
+#include "row_ops.cuh"
+
+namespace f2s {
+namespace {
+
+using namespace rows;
+
+constexpr int kMaxK = 131071;
+
+struct Int8Args {
+    const int8_t* x;
+    int64_t ldx;
+    const float* xs;
+    const int8_t* w;
+    int64_t ldw;
+    const float* ws;
+    const void* bias;  // of y's type, or null
+    void* y;
+    int64_t ldy;
+    int rows, cols, K;
+};
+
+// Any pitch and alignment: 64 x 64 outputs per block of 256 threads, 4 x 4
+// each, K in steps of 64 staged in shared memory as words of four, four
+// products and sums per dp4a.
+template <typename T>
+__global__ void __launch_bounds__(256) linear_int8_any_kernel(const Int8Args g) {
+    __shared__ int8_t xa[64][68], wa[64][68];
+    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    int acc[4][4] = {};
+    for (int k0 = 0; k0 < g.K; k0 += 64) {
+        for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+            const int r = i / 64, k = i % 64;
+            const bool in = k0 + k < g.K;
+            xa[r][k] = in && m0 + r < g.rows ? g.x[(m0 + r) * g.ldx + k0 + k] : (int8_t)0;
+            wa[r][k] = in && n0 + r < g.cols ? g.w[(n0 + r) * g.ldw + k0 + k] : (int8_t)0;
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int k = 0; k < 64; k += 4) {
+            int a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = *reinterpret_cast<const int*>(&xa[ty + 16 * i][k]);
+                b[i] = *reinterpret_cast<const int*>(&wa[tx + 16 * i][k]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(a[i], b[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int m = m0 + ty + 16 * i;
+        if (m >= g.rows) continue;
+        const float xs = g.xs[m];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = n0 + tx + 16 * j;
+            if (n >= g.cols) continue;
+            const float b = g.bias ? to_f32<T>(static_cast<const T*>(g.bias)[n]) : 0.0f;
+            static_cast<T*>(g.y)[m * g.ldy + n] = from_f32<T>(fmaf((float)acc[i][j] * xs, g.ws[n], b));
+        }
+    }
+}
+
+template <typename T>
+int any_launch(const Int8Args& g, cudaStream_t st) {
+    F2S_LIMIT(ceil_div(g.rows, 64) <= 65535, "linear_int8: %d rows of an unaligned pitch", g.rows);
+    linear_int8_any_kernel<T><<<dim3(ceil_div(g.cols, 64), ceil_div(g.rows, 64)), 256, 0, st>>>(g);
+    return check_launch("linear_int8_any_kernel");
+}
+
+}  // namespace
+}  // namespace f2s
+
+extern "C" int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+                               const float* w_scale, const void* bias, void* y, int64_t ldy, int dtype, int rows,
+                               int cols, int K, void* stream) {
+    F2S_TRY(f2s::rows::check_dtype("linear_int8", dtype));
+    F2S_REQUIRE(rows >= 0 && cols >= 1 && K >= 1, "linear_int8: bad shape rows=%d cols=%d K=%d", rows, cols, K);
+    F2S_LIMIT(K <= f2s::kMaxK, "linear_int8: K=%d, at most %d for an exact 32-bit sum", K, f2s::kMaxK);
+    if (rows == 0) return F2S_OK;
+    F2S_REQUIRE(x && x_scale && w && w_scale && y, "linear_int8: null pointer");
+    F2S_REQUIRE(ldx >= K && ldw >= K && ldy >= cols, "linear_int8: row pitch below the row");
+    f2s::Int8Args g{x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, rows, cols, K};
+    cudaStream_t st = f2s::as_stream(stream);
+    f2s::TraceScope trace(f2s::kTagGemmInt8, st);
+    int status = F2S_OK;
+    F2S_DTYPE_SWITCH(dtype, status = f2s::any_launch<T>(g, st));
+    return status;
+}

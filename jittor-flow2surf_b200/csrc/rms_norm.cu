@@ -1,0 +1,364 @@
+// Root-mean-square norm of a residual stream, with the residual's addition:
+//   s = x + r (rounded to the stream's type, as it is stored)
+//   y = s rstd w,  rstd = (mean(s^2) + eps)^-1/2
+// and its backward, or y as 8-bit rows with one scale each:
+//   q = rint(127 s w / m), m = max |s w|, scale = m rstd / 127.
+// rstd cancels in q, so the sum and the maximum come from one reduction and q
+// is the exact rounding whatever the order of the sum.
+//
+// All are bound by memory: the forward reads x, r and writes s, y (8 bytes per
+// channel in 16 bits, 7 with 8-bit rows), the backward reads s, dy, ds and
+// writes dx (8 bytes). Rows are held in registers (row_ops.cuh), so each is
+// read once.
+#include <type_traits>
+
+#include "kernels.cuh"
+#include "row_ops.cuh"
+
+namespace f2s {
+namespace {
+
+using namespace rows;
+
+struct NormArgs {
+    const void* x;
+    int64_t ldx;
+    const void* residual;  // null: none (s = x, `stream` not written)
+    int64_t ldr;
+    const void* weight;
+    int64_t nrows;
+    int C;
+    float eps;
+    void* stream;  // (nrows, C)
+    void* y;       // (nrows, C), or
+    int8_t* q;     // 8-bit rows of pitch ldq
+    int64_t ldq;
+    float* scale;
+};
+
+__device__ __forceinline__ float reciprocal_rms(float sum, int C, float eps) {
+    return __frsqrt_rn(sum / (float)C + eps);
+}
+
+// k8: 8-bit rows. The products s w of a 16-bit type are exact in fp32; those of
+// fp32 are taken in 64 bits for the maximum and at rounding borders.
+template <typename T, int E, int TPR, bool kWide, bool k8>
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR)
+add_rms_norm_kernel(const NormArgs g) {
+    using S = Slice<T, E, TPR, kWide>;
+    constexpr bool kExact64 = k8 && sizeof(T) == 4;
+    using M = typename std::conditional<kExact64, unsigned long long, uint32_t>::type;
+    __shared__ M shared_m[32];
+    __shared__ float shared_a[32];
+    const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
+    const int64_t row = TPR <= 32 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
+    // rows past the end take part in the shuffles and write nothing
+    const bool live = row < g.nrows;
+    const int C = live ? g.C : 0;
+    float s[E], w[E];
+    S::load(static_cast<const T*>(g.x) + (live ? row : 0) * g.ldx, C, t, s);
+    if (g.residual) {
+        float r[E];
+        S::load(static_cast<const T*>(g.residual) + (live ? row : 0) * g.ldr, C, t, r);
+        S::load(static_cast<const T*>(g.weight), C, t, w);
+#pragma unroll
+        for (int i = 0; i < E; ++i) s[i] = rounded<T>(s[i] + r[i]);
+        S::store(static_cast<T*>(g.stream) + (live ? row : 0) * (int64_t)g.C, C, t, s);
+    } else {
+        S::load(static_cast<const T*>(g.weight), C, t, w);
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum = fmaf(s[i], s[i], sum);
+    M m = 0;
+    if constexpr (k8) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            M b;
+            if constexpr (kExact64)
+                b = (unsigned long long)__double_as_longlong(fabs((double)s[i] * (double)w[i]));
+            else b = abs_bits(s[i] * w[i]);
+            m = b > m ? b : m;
+        }
+    }
+    row_sum_max<TPR>(sum, m, shared_m, shared_a);
+    const float rstd = reciprocal_rms(sum, g.C, g.eps);
+    if constexpr (k8) {
+        double largest;
+        bool finite;
+        if constexpr (kExact64) {
+            largest = __longlong_as_double((long long)m);
+            finite = m < kInfBits64 && largest < 3.0e38;
+        } else {
+            largest = (double)__uint_as_float(m);
+            finite = m < kInfBits;
+        }
+        const float lf = (float)largest;
+        const float inv = 127.0f / lf;
+        float p[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) p[i] = s[i] * w[i];
+        uint32_t q[E];
+        round8_row(p, inv, finite ? largest : 0.0, finite && lf >= kTiny, q,
+                   [&](int i) { return (double)s[i] * (double)w[i]; });
+        S::store8(g.q + (live ? row : 0) * g.ldq, C, t, q);
+        if (live && t == 0)
+            g.scale[row] = finite ? (float)(largest / 127.0 * (double)rstd) : __int_as_float(0x7fc00000);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s[i] = s[i] * rstd * w[i];
+        S::store(static_cast<T*>(g.y) + (live ? row : 0) * (int64_t)g.C, C, t, s);
+    }
+}
+
+template <bool k8>
+int norm_launch(const NormArgs& g, int dtype, cudaStream_t st) {
+    const int size = dtype_size(dtype), vec = 16 / size;
+    const bool wide = g.C % vec == 0 && aligned16(g.x) && (g.ldx % vec == 0 || g.nrows == 1) && aligned16(g.weight) &&
+                      (!g.residual || (aligned16(g.residual) && (g.ldr % vec == 0 || g.nrows == 1) && aligned16(g.stream))) &&
+                      (k8 ? (aligned16(g.q) && (g.ldq % vec == 0 || g.nrows == 1)) : aligned16(g.y));
+    const Shape s = pick_shape(g.nrows, g.C, wide);
+    const int64_t blocks = ceil_div64(g.nrows, block_rows(s.tpr));
+    F2S_LIMIT(blocks <= INT32_MAX, "add_rms_norm: %lld rows", (long long)g.nrows);
+    TraceScope trace(kTagRmsNorm, st);
+#define F2S_LAUNCH(T, E, TPR, W) \
+    add_rms_norm_kernel<T, E, TPR, W, k8><<<(unsigned)blocks, block_threads(TPR), 0, st>>>(g)
+    F2S_DTYPE_SWITCH(dtype, F2S_ROW_DISPATCH(s, wide, T, F2S_LAUNCH));
+#undef F2S_LAUNCH
+    return check_launch("add_rms_norm_kernel");
+}
+
+// ---- backward ---------------------------------------------------------------
+// With u = dy w and n = s rstd:
+//   dx = ds + rstd (u - n mean(u n)),   dw = sum over rows of dy n.
+// Blocks walk the rows by the grid and keep their part of dw in registers
+// (32-bit sums in a fixed order: per thread over its rows, over the block's
+// row groups, then over the blocks by weight_grad_kernel), so it costs one
+// (blocks x C) array instead of another pass over dy and s.
+struct NormGradArgs {
+    const void* s;
+    int64_t lds;
+    const void* weight;
+    const void* dy;
+    int64_t lddy;
+    const void* ds;  // gradient of the stream output, or null
+    int64_t ldds;
+    int64_t nrows;
+    int C;
+    float eps;
+    void* dx;        // (nrows, C)
+    float* partial;  // (blocks, C), or null: no weight gradient
+};
+
+template <typename T, int E, int TPR, bool kWide>
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR)
+add_rms_norm_grad_kernel(const NormGradArgs g) {
+    using S = Slice<T, E, TPR, kWide>;
+    constexpr int kRows = TPR <= 32 ? 256 / TPR : 1;
+    __shared__ float shared_a[2][32], shared_b[2][32];
+    const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
+    const int group = TPR <= 32 ? threadIdx.x / TPR : 0;
+    float dw[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) dw[i] = 0.0f;
+    int parity = 0;
+    for (int64_t first = (int64_t)blockIdx.x * kRows; first < g.nrows; first += (int64_t)gridDim.x * kRows) {
+        const int64_t row = first + group;
+        const bool live = row < g.nrows;
+        const int64_t at = live ? row : 0;
+        const int C = live ? g.C : 0;
+        float s[E], dy[E], w[E];
+        S::load(static_cast<const T*>(g.s) + at * g.lds, C, t, s);
+        S::load(static_cast<const T*>(g.dy) + at * g.lddy, C, t, dy);
+        S::load(static_cast<const T*>(g.weight), C, t, w);
+        float sum = 0.0f, along = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            sum = fmaf(s[i], s[i], sum);
+            w[i] *= dy[i];
+            along = fmaf(w[i], s[i], along);
+        }
+        constexpr int kWidth = TPR < 32 ? TPR : 32;
+#pragma unroll
+        for (int o = kWidth / 2; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            along += __shfl_xor_sync(0xffffffffu, along, o);
+        }
+        if constexpr (TPR > 32) {
+            // two buffers by turns: a row's partial sums are read before the
+            // barrier of the next row, and overwritten only after it
+            constexpr int kWarps = TPR / 32;
+            const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+            if (lane == 0) {
+                shared_a[parity][warp] = sum;
+                shared_b[parity][warp] = along;
+            }
+            __syncthreads();
+            sum = lane < kWarps ? shared_a[parity][lane] : 0.0f;
+            along = lane < kWarps ? shared_b[parity][lane] : 0.0f;
+#pragma unroll
+            for (int o = kWarps / 2; o > 0; o >>= 1) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                along += __shfl_xor_sync(0xffffffffu, along, o);
+            }
+            sum = __shfl_sync(0xffffffffu, sum, 0);
+            along = __shfl_sync(0xffffffffu, along, 0);
+            parity ^= 1;
+        }
+        // 0 past the last row: with eps = 0 its reciprocal would put NaN into dw
+        const float rstd = live ? reciprocal_rms(sum, g.C, g.eps) : 0.0f;
+        const float mean = along * rstd / (float)g.C;  // mean(u n)
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float n = s[i] * rstd;
+            dw[i] = fmaf(dy[i], n, dw[i]);
+            s[i] = rstd * (w[i] - n * mean);
+        }
+        if (g.ds) {
+            float ds[E];
+            S::load(static_cast<const T*>(g.ds) + at * g.ldds, C, t, ds);
+#pragma unroll
+            for (int i = 0; i < E; ++i) s[i] += ds[i];
+        }
+        S::store(static_cast<T*>(g.dx) + at * (int64_t)g.C, C, t, s);
+    }
+    if (!g.partial) return;
+    float* mine = g.partial + (int64_t)blockIdx.x * g.C;
+    if constexpr (TPR <= 32) {
+        // the block's row groups, in order: the groups of a warp by shuffles,
+        // then the warps through shared memory
+#pragma unroll
+        for (int o = TPR; o < 32; o <<= 1) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
+        }
+        __shared__ float sums[8][TPR * E];
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        if (lane < TPR) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) sums[warp][S::channel(i, t)] = dw[i];
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < g.C; c += 256) {
+            float a = sums[0][c];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) a += sums[k][c];
+            mine[c] = a;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int c = S::channel(i, t);
+            if (c < g.C) mine[c] = dw[i];
+        }
+    }
+}
+
+// dw[c] = sum over blocks of partial[block][c]: 32 channels x 8 slices of the
+// blocks per CTA.
+template <typename T>
+__global__ void __launch_bounds__(256) weight_grad_kernel(const float* __restrict__ partial, int blocks, int C,
+                                                          T* __restrict__ dw) {
+    __shared__ float sums[8][32];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;
+    float a = 0.0f;
+    if (c < C)
+        for (int b = slice; b < blocks; b += 8) a += partial[(int64_t)b * C + c];
+    sums[slice][lane] = a;
+    __syncthreads();
+    if (slice == 0 && c < C) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) a += sums[k][lane];
+        dw[c] = from_f32<T>(a);
+    }
+}
+
+template <typename T>
+void weight_grad_launch(const float* partial, int blocks, int C, void* dw, cudaStream_t st) {
+    weight_grad_kernel<T><<<ceil_div(C, 32), 256, 0, st>>>(partial, blocks, C, static_cast<T*>(dw));
+}
+
+// Blocks of the backward: enough to fill the SMs, each with several rows to
+// share its dw over.
+int grad_blocks(int64_t nrows, int C) {
+    const Shape s = pick_shape(nrows, C, true);
+    const int64_t all = ceil_div64(nrows, block_rows(s.tpr));
+    const int per_sm = s.tpr <= 32 ? 4 : s.tpr == 128 ? 8 : 2;
+    const int64_t most = (int64_t)sm_count() * per_sm;
+    return (int)(all < most ? all : most);
+}
+
+int check_norm(const char* what, int dtype, int64_t nrows, int C, float eps) {
+    F2S_TRY(check_dtype(what, dtype));
+    F2S_REQUIRE(nrows >= 0 && C >= 1 && eps >= 0.0f, "%s: bad shape rows=%lld C=%d eps=%g", what,
+                (long long)nrows, C, (double)eps);
+    F2S_LIMIT(C <= kMaxRow, "%s: C=%d, at most %d channels", what, C, kMaxRow);
+    return F2S_OK;
+}
+
+}  // namespace
+}  // namespace f2s
+
+extern "C" int f2s_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                                int dtype, int64_t rows, int C, float eps, void* stream_out, void* y, void* stream) {
+    F2S_TRY(f2s::check_norm("add_rms_norm", dtype, rows, C, eps));
+    if (rows == 0) return F2S_OK;
+    F2S_REQUIRE(x && weight && y && (!residual || stream_out), "add_rms_norm: null pointer");
+    F2S_REQUIRE(ldx >= C && (!residual || ldr >= C), "add_rms_norm: row pitch below C=%d", C);
+    f2s::NormArgs g{x, ldx, residual, ldr, weight, rows, C, eps, stream_out, y, nullptr, 0, nullptr};
+    return f2s::norm_launch<false>(g, dtype, f2s::as_stream(stream));
+}
+
+extern "C" int f2s_add_rms_norm_int8(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                     const void* weight, int dtype, int64_t rows, int C, float eps, void* stream_out,
+                                     int8_t* q, int64_t ldq, float* scale, void* stream) {
+    F2S_TRY(f2s::check_norm("add_rms_norm_int8", dtype, rows, C, eps));
+    if (rows == 0) return F2S_OK;
+    F2S_REQUIRE(x && weight && q && scale && (!residual || stream_out), "add_rms_norm_int8: null pointer");
+    F2S_REQUIRE(ldx >= C && ldq >= C && (!residual || ldr >= C), "add_rms_norm_int8: row pitch below C=%d", C);
+    f2s::NormArgs g{x, ldx, residual, ldr, weight, rows, C, eps, stream_out, nullptr, q, ldq, scale};
+    return f2s::norm_launch<true>(g, dtype, f2s::as_stream(stream));
+}
+
+extern "C" int f2s_add_rms_norm_backward_workspace_bytes(int64_t rows, int C, size_t* bytes) {
+    F2S_TRY(f2s::check_norm("add_rms_norm_backward", F2S_DTYPE_F32, rows, C, 0.0f));
+    F2S_REQUIRE(bytes, "add_rms_norm_backward: null pointer");
+    *bytes = (size_t)f2s::grad_blocks(rows, C) * C * sizeof(float);
+    return F2S_OK;
+}
+
+extern "C" int f2s_add_rms_norm_backward(const void* s, int64_t lds, const void* weight, int dtype, int64_t rows,
+                                         int C, float eps, const void* dy, int64_t lddy, const void* ds, int64_t ldds,
+                                         void* dx, void* dweight, void* workspace, size_t workspace_bytes,
+                                         void* stream) {
+    using namespace f2s;
+    using namespace f2s::rows;
+    F2S_TRY(check_norm("add_rms_norm_backward", dtype, rows, C, eps));
+    cudaStream_t st = as_stream(stream);
+    if (rows == 0) {
+        if (dweight) F2S_CUDA_TRY(cudaMemsetAsync(dweight, 0, (size_t)C * dtype_size(dtype), st));
+        return F2S_OK;
+    }
+    F2S_REQUIRE(s && weight && dy && dx, "add_rms_norm_backward: null pointer");
+    F2S_REQUIRE(lds >= C && lddy >= C && (!ds || ldds >= C), "add_rms_norm_backward: row pitch below C=%d", C);
+    const int blocks = grad_blocks(rows, C);
+    if (dweight && (!workspace || workspace_bytes < (size_t)blocks * C * sizeof(float)))
+        return fail(F2S_ERR_WORKSPACE, "add_rms_norm_backward: workspace of %zu bytes, %zu needed", workspace_bytes,
+                    (size_t)blocks * C * sizeof(float));
+    const int vec = 16 / dtype_size(dtype);
+    auto pitched = [&](const void* p, int64_t ld) { return aligned16(p) && (ld % vec == 0 || rows == 1); };
+    const bool wide = C % vec == 0 && pitched(s, lds) && pitched(dy, lddy) && (!ds || pitched(ds, ldds)) &&
+                      aligned16(weight) && aligned16(dx);
+    NormGradArgs g{s, lds, weight, dy, lddy, ds, ldds, rows, C, eps, dx, dweight ? static_cast<float*>(workspace) : nullptr};
+    const Shape shape = pick_shape(rows, C, wide);
+    TraceScope trace(kTagRmsNorm, st);
+#define F2S_LAUNCH(T, E, TPR, W) \
+    add_rms_norm_grad_kernel<T, E, TPR, W><<<blocks, block_threads(TPR), 0, st>>>(g)
+    F2S_DTYPE_SWITCH(dtype, F2S_ROW_DISPATCH(shape, wide, T, F2S_LAUNCH));
+#undef F2S_LAUNCH
+    F2S_TRY(check_launch("add_rms_norm_grad_kernel"));
+    if (!dweight) return F2S_OK;
+    F2S_DTYPE_SWITCH(dtype, weight_grad_launch<T>(static_cast<const float*>(workspace), blocks, C, dweight, st));
+    return check_launch("weight_grad_kernel");
+}

@@ -62,6 +62,17 @@ SIGNATURES: dict[str, list] = {
     "f2s_point_to_mesh_workspace_bytes": [_i, _i, _p],
     "f2s_point_to_mesh": [_p, _i, _p, _i, _p, _i, _p, _p, _p, _sz, _p],
     "f2s_linear": [_p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+    "f2s_add_rms_norm": [_p, _i64, _p, _i64, _p, _i, _i64, _i, _f, _p, _p, _p],
+    "f2s_add_rms_norm_int8": [_p, _i64, _p, _i64, _p, _i, _i64, _i, _f, _p, _p, _i64, _p, _p],
+    "f2s_add_rms_norm_backward_workspace_bytes": [_i64, _i, _p],
+    "f2s_add_rms_norm_backward": [_p, _i64, _p, _i, _i64, _i, _f, _p, _i64, _p, _i64, _p, _p, _p,
+                                  _sz, _p],
+    "f2s_quantize_rows": [_p, _i64, _i, _i64, _i, _p, _i64, _p, _p],
+    "f2s_dequantize_rows": [_p, _i64, _p, _i64, _i, _p, _i64, _i, _p],
+    "f2s_linear_int8": [_p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i, _i, _i, _i, _p],
+    "f2s_swiglu": [_p, _i64, _i, _i64, _i, _p, _p, _p, _p],
+    "f2s_swiglu_backward": [_p, _i64, _p, _p, _p, _i64, _i, _i64, _i, _p, _p],
+    "f2s_swiglu_int8": [_p, _i64, _i, _i64, _i, _p, _i64, _p, _p],
     "f2s_device_error": [_p, _i, _p],
     "f2s_selftest_wait_timeout": [_i, _p],
     "f2s_nearest_backward": [_p, _p, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p],
