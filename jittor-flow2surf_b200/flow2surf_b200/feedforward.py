@@ -57,13 +57,28 @@ def _same_device(first: torch.Tensor, *others) -> None:
             raise ValueError(f"tensors lie on different devices: {first.device} and {t.device}")
 
 
+_ENTRIES: dict = {}  # name -> entry point of the loaded library
+
+
 def _call(device: torch.device, name: str, *args) -> None:
-    """Launch on `device`'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    """Launch on `device`'s current stream, whichever device is current. (The
+    stream's handle is asked for directly: building a Stream object for it
+    takes longer than a launch.)"""
+    entry = _ENTRIES.get(name)
+    if entry is None:
+        entry = _ENTRIES[name] = getattr(_lib.lib(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)
+
+
+def _empty(like: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 class Int8Rows(NamedTuple):
@@ -79,7 +94,7 @@ class Int8Rows(NamedTuple):
         """What the rows stand for, in `dtype`."""
         code = _dtype(dtype)
         values, scale = _check_int8("rows", self)
-        out = torch.empty(values.shape, dtype=dtype, device=values.device)
+        out = torch.empty_like(values, dtype=dtype, memory_format=torch.contiguous_format)
         if out.numel() == 0:
             return out
         values, rows, pitch = _rows(values)
@@ -103,15 +118,17 @@ def _check_int8(name: str, rows: Int8Rows):
     return values, scale if scale.is_contiguous() else scale.contiguous()
 
 
-def _empty_int8(shape, device) -> tuple[Int8Rows, int]:
-    """Unset 8-bit rows (..., channels) and their pitch, a multiple of 16."""
-    *lead, width = shape
+def _empty_int8(like: torch.Tensor, width: int | None = None) -> tuple[Int8Rows, int]:
+    """Unset 8-bit rows with the leading shape of `like` (its width unless given)
+    and their pitch, a multiple of 16."""
+    lead = like.shape[:-1]
+    if width is None:
+        width = like.shape[-1]
     pitch = -(-width // 16) * 16
-    if pitch == width:
-        values = torch.empty(shape, dtype=torch.int8, device=device)
-    else:
-        values = torch.empty((*lead, pitch), dtype=torch.int8, device=device)[..., :width]
-    return Int8Rows(values, torch.empty(lead, dtype=torch.float32, device=device)), pitch
+    values = like.new_empty((*lead, pitch), dtype=torch.int8)
+    if pitch != width:
+        values = values[..., :width]
+    return Int8Rows(values, like.new_empty(lead, dtype=torch.float32)), pitch
 
 
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
@@ -125,7 +142,7 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     _require_cuda(x)
     if _needs_grad(x):
         raise ValueError("8-bit rows have no gradient; call quantize_rows under torch.no_grad()")
-    out, pitch = _empty_int8(x.shape, x.device)
+    out, pitch = _empty_int8(x)
     if x.numel() == 0:
         return out
     x, rows, ldx = _rows(x)
@@ -158,7 +175,7 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
             raise ValueError("the 8-bit product has no gradient; call linear_int8 under "
                              "torch.no_grad()")
         bias = bias.contiguous()
-    out = torch.empty((*xv.shape[:-1], cols), dtype=dtype, device=xv.device)
+    out = xv.new_empty((*xv.shape[:-1], cols), dtype=dtype)
     if out.numel() == 0:
         return out
     xv, rows, ldx = _rows(xv)
@@ -206,8 +223,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
 
 
 def _norm_forward(x, weight, residual, eps, code):
-    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stream = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    normed = _empty(x)
+    stream = x if residual is None else _empty(x)
     if x.numel() == 0:
         return normed, stream
     width = x.shape[-1]
@@ -244,8 +261,8 @@ class _AddRmsNorm(torch.autograd.Function):
             return (dstream if need_x else None, torch.zeros_like(weight) if need_weight else None,
                     dstream if need_residual else None, None, None)
         width = stream.shape[-1]
-        dx = torch.empty(stream.shape, dtype=stream.dtype, device=stream.device)
-        dweight = torch.empty(width, dtype=weight.dtype, device=weight.device) if need_weight else None
+        dx = _empty(stream)
+        dweight = _empty(weight) if need_weight else None
         if stream.numel() == 0:
             return (dx if need_x else None, dweight.zero_() if need_weight else None,
                     dx if need_residual else None, None, None)
@@ -259,7 +276,7 @@ class _AddRmsNorm(torch.autograd.Function):
         ws, size = None, ctypes.c_size_t(0)
         if need_weight:
             _lib.call("f2s_add_rms_norm_backward_workspace_bytes", rows, width, ctypes.byref(size))
-            ws = torch.empty(size.value, dtype=torch.uint8, device=s.device)
+            ws = s.new_empty(size.value, dtype=torch.uint8)
         _call(s.device, "f2s_add_rms_norm_backward", s.data_ptr(), lds, weight.data_ptr(), ctx.code,
               rows, width, ctx.eps, dy.data_ptr(), lddy, ds, ldds, dx.data_ptr(),
               None if dweight is None else dweight.data_ptr(),
@@ -277,8 +294,8 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
     if _needs_grad(x, weight) or (residual is not None and _needs_grad(residual)):
         raise ValueError("8-bit rows have no gradient; call add_rms_norm_int8 under "
                          "torch.no_grad(), or add_rms_norm")
-    out, pitch = _empty_int8(x.shape, x.device)
-    stream = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out, pitch = _empty_int8(x)
+    stream = x if residual is None else _empty(x)
     if x.numel() == 0:
         return out, stream
     width = x.shape[-1]
@@ -321,8 +338,7 @@ def swiglu(projected: torch.Tensor, *, checkpoint: str | None = None) -> torch.T
 
 def _swiglu_forward(projected, code, kept, scales):
     hidden = projected.shape[-1] // 2
-    out = torch.empty((*projected.shape[:-1], hidden), dtype=projected.dtype,
-                      device=projected.device)
+    out = projected.new_empty((*projected.shape[:-1], hidden))
     if out.numel() == 0:
         return out
     p, rows, ld = _rows(projected)
@@ -342,15 +358,15 @@ class _SwiGlu(torch.autograd.Function):
             ctx.save_for_backward(projected)
             return _swiglu_forward(projected, code, None, None)
         groups = projected.numel() // (2 * hidden) * -(-hidden // _SWIGLU_GROUP)
-        kept = torch.empty(groups * 2 * _SWIGLU_GROUP, dtype=torch.int8, device=projected.device)
-        scales = torch.empty(2 * groups, dtype=torch.float32, device=projected.device)
+        kept = projected.new_empty(groups * 2 * _SWIGLU_GROUP, dtype=torch.int8)
+        scales = projected.new_empty(2 * groups, dtype=torch.float32)
         ctx.save_for_backward(kept, scales)
         return _swiglu_forward(projected, code, kept, scales)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        grad = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device)
+        grad = dy.new_empty(ctx.shape)
         if grad.numel() == 0:
             return grad, None, None
         hidden = ctx.shape[-1] // 2
@@ -375,7 +391,7 @@ def swiglu_int8(projected: torch.Tensor) -> Int8Rows:
         raise ValueError("8-bit rows have no gradient; call swiglu_int8 under torch.no_grad(), "
                          "or swiglu")
     hidden = projected.shape[-1] // 2
-    out, pitch = _empty_int8((*projected.shape[:-1], hidden), projected.device)
+    out, pitch = _empty_int8(projected, hidden)
     if out.values.numel() == 0:
         return out
     p, rows, ld = _rows(projected)
