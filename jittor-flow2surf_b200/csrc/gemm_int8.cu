@@ -1,0 +1,658 @@
+// Tensor-core forms of the 8-bit product (tcgen05 kind::i8, exact 32-bit
+// sums): y[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k] + b[n].
+//
+// tiles  few tokens, or few tiles: one CTA per 128 channels x BN tokens, the
+//        weights as the M = 128 operand (their bytes are what bounds the call),
+//        K split over the CTAs of a cluster, which add their integer sums
+//        through shared memory: the result does not depend on the split.
+// pairs  many tokens: persistent CTA pairs (cta_group::2) on 256 x bn tiles.
+//        Each CTA stages its 128 token rows and half of the channels, so a
+//        pair moves 32 KB per 128-byte K block and SM where single CTAs of
+//        128 x 256 would move 48 KB, more than L2 delivers at the int8 rate.
+//
+// Operands come by TMA in 128-byte rows (K blocks of 128) with the 128-byte
+// swizzle; columns past K and rows past the matrix read as zeros.
+#include "gemm_int8.cuh"
+#include "row_ops.cuh"
+#include "tc_common.cuh"
+
+namespace f2s {
+namespace {
+
+using rows::from_f32;
+using rows::to_f32;
+
+constexpr size_t kSmemLimit = 227 * 1024;
+constexpr int kBlockK = 128;
+
+// Instruction descriptor of kind::i8: 32-bit integer sums, both operands
+// signed and K-major.
+constexpr uint32_t idesc_i8(int M, int N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// ---- clusters ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Address of this CTA's shared address `a` in the CTA of cluster rank `r`.
+__device__ __forceinline__ uint32_t map_rank(uint32_t a, uint32_t r) {
+    uint32_t d;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(r));
+    return d;
+}
+__device__ __forceinline__ void store_cluster(uint32_t a, int v) {
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ float bias_at(const void* bias, int n) {
+    return bias ? to_f32<T>(static_cast<const T*>(bias)[n]) : 0.0f;
+}
+
+// ---- tiles -------------------------------------------------------------------
+
+struct TileArgs {
+    const float* xs;
+    const float* ws;
+    const void* bias;
+    void* y;
+    int64_t ldy;
+    int rows, cols;
+    int k_blocks, stages, split;
+    int* err;
+};
+
+constexpr int kTileThreads = 192;  // TMA warp, MMA warp, 4 epilogue warps
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kTileThreads)
+linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                         const TileArgs g) {
+    constexpr uint32_t kA = 128 * 128, kB = BN * 128, kStage = kA + kB;
+    constexpr uint32_t kCols = BN < 32 ? 32 : BN;
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int S = g.stages;
+    int* partial = reinterpret_cast<int*>(smem + (size_t)S * kStage);  // [split][BN / split][128]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * kStage + (g.split > 1 ? BN * 512 : 0));
+    uint64_t* empty = full + S;
+    uint64_t* done = empty + S;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = g.split;
+    const int rank = (int)blockIdx.x % split;
+    const int n0 = (int)blockIdx.x / split * 128, m0 = (int)blockIdx.y * BN;
+    const int kb0 = (int)((int64_t)rank * g.k_blocks / split);
+    const int kb1 = (int)((int64_t)(rank + 1) * g.k_blocks / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            tc::mbar_init(&full[s], 1);
+            tc::mbar_init(&empty[s], 1);
+        }
+        tc::mbar_init(done, 1);
+        tc::fence_barrier_init();
+        tc::prefetch_tensormap(&map_w);
+        tc::prefetch_tensormap(&map_x);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_slot, kCols);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // the other CTAs write into this one's `partial` only once it has started
+    if (split > 1) cluster_arrive();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t pending = 0, pending_phase = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const int i = kb - kb0, s = i % S;
+                const uint32_t phase = (uint32_t)(i / S) & 1u;
+                if (!tc::mbar_wait(&empty[s], phase ^ 1u, g.err)) {
+                    ok = false;
+                    break;
+                }
+                unsigned char* st = smem + (size_t)s * kStage;
+                tc::mbar_arrive_expect_tx(&full[s], kStage);
+                tc::tma_load_2d(st, &map_w, &full[s], kb * kBlockK, n0);
+                tc::tma_load_2d(st + kA, &map_x, &full[s], kb * kBlockK, m0);
+                pending |= 1u << s;
+                pending_phase = (pending_phase & ~(1u << s)) | (phase << s);
+            }
+            if (!ok) {
+                // let the copies already issued land before the CTA exits
+                for (int s = 0; s < S; ++s)
+                    if (pending & (1u << s)) tc::mbar_drain(&full[s], (pending_phase >> s) & 1u);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const int i = kb - kb0, s = i % S;
+                if (!tc::mbar_wait_poll(&full[s], (uint32_t)(i / S) & 1u, g.err)) break;
+                tc::tc_fence_after();
+                const uint32_t st = tc::smem_u32(smem + (size_t)s * kStage);
+                const uint64_t a = tc::sw128_desc(st), b = tc::sw128_desc(st + kA);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_i8(tmem, a + 2 * k, b + 2 * k, idesc_i8(128, BN), (i | k) ? 1u : 0u);
+                tc::umma_commit(&empty[s]);
+            }
+            // every MMA issued has completed (TMEM is freed below)
+            tc::umma_commit(done);
+            tc::mbar_drain(done, 0);
+        }
+        __syncwarp();
+    }
+    if (split > 1) cluster_wait();
+    bool ok = true;
+    const int channel = (warp & 3) * 32 + lane;  // a warp reads its TMEM lane quarter
+    const int n = n0 + channel;
+    constexpr int kStep = BN < 32 ? 16 : 32;
+    auto store = [&](int m, int acc, float ws, float b) {
+        static_cast<T*>(g.y)[m * g.ldy + n] = from_f32<T>(fmaf((float)acc * __ldg(g.xs + m), ws, b));
+    };
+    float ws = 0.0f, b = 0.0f;
+    if (warp >= 2) {
+        if (n < g.cols) {
+            ws = __ldg(g.ws + n);
+            b = bias_at<T>(g.bias, n);
+        }
+        ok = __all_sync(0xffffffffu, tc::mbar_wait_poll(done, 0, g.err));
+        tc::tc_fence_after();
+        const int own = BN / split;  // tokens that each CTA of the cluster finishes
+        const int shift = __ffs(own) - 1;
+        const uint32_t mine = tc::smem_u32(partial + rank * own * 128 + channel);
+#pragma unroll
+        for (int j0 = 0; j0 < BN; j0 += kStep) {
+            uint32_t v[kStep];
+            const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + j0;
+            if constexpr (kStep == 32) {
+                tc::tmem_ld32_issue(from, v);
+                tc::tmem_ld32_wait(v);
+            } else {
+                tc::tmem_ld16_issue(from, v);
+                tc::tmem_ld16_wait(v);
+            }
+            if (!ok) continue;
+            if (split == 1) {
+                if (n < g.cols) {
+#pragma unroll
+                    for (int j = 0; j < kStep; ++j)
+                        if (m0 + j0 + j < g.rows) store(m0 + j0 + j, (int)v[j], ws, b);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kStep; ++j) {
+                    const uint32_t to = (uint32_t)(j0 + j) >> shift;
+                    store_cluster(map_rank(mine + ((uint32_t)(j0 + j) & (own - 1)) * 512u, to), (int)v[j]);
+                }
+            }
+        }
+    }
+    if (split > 1) {
+        cluster_arrive();
+        cluster_wait();
+        if (warp >= 2 && ok && n < g.cols) {
+            const int own = BN / split;
+            for (int j = 0; j < own; ++j) {
+                const int m = m0 + rank * own + j;
+                if (m >= g.rows) break;
+                int acc = 0;
+                for (int r = 0; r < split; ++r) acc += partial[(r * own + j) * 128 + channel];
+                store(m, acc, ws, b);
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 1) tc::tmem_dealloc(tmem, kCols);
+}
+
+int operand_map(CUtensorMap* map, const int8_t* p, int64_t ld, int nrows, int K, int box_rows) {
+    // one row has no pitch of its own
+    return make_tensor_map_2d_typed(map, p, kTmaU8, 128, nrows, K, nrows == 1 ? ceil_div64(K, 16) * 16 : ld, box_rows,
+                                    kBlockK);
+}
+
+template <typename T, int BN>
+int tiles_launch(const Int8Args& a, int split, cudaStream_t st) {
+    CUtensorMap mw, mx;
+    F2S_TRY(operand_map(&mw, a.w, a.ldw, a.cols, a.K, 128));
+    F2S_TRY(operand_map(&mx, a.x, a.ldx, a.rows, a.K, BN));
+    TileArgs g{a.xs, a.ws, a.bias, a.y, a.ldy, a.rows, a.cols, ceil_div(a.K, kBlockK), 0, split, tc_error_word()};
+    if (!g.err) return fail(F2S_ERR_CUDA, "linear_int8: device error word unavailable");
+    const size_t stage = 128 * 128 + BN * 128;
+    const size_t fixed = 1024 + 512 + (split > 1 ? BN * 512 : 0);
+    // two CTAs per SM where there are that many
+    const int per_cta = ceil_div(g.k_blocks, split);
+    const int64_t ctas = (int64_t)ceil_div(a.cols, 128) * split * ceil_div(a.rows, BN);
+    const size_t budget = BN < 128 && ctas > sm_count() ? kSmemLimit / 2 - 1024 : kSmemLimit;
+    int stages = (int)((budget - fixed) / stage);
+    stages = stages < 12 ? stages : 12;
+    stages = stages < per_cta ? stages : per_cta;
+    g.stages = stages;
+    const size_t smem = fixed + stages * stage;
+    auto kernel = linear_int8_tiles_kernel<T, BN>;
+    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int token_tiles = ceil_div(a.rows, BN);
+    F2S_LIMIT(token_tiles <= 65535, "linear_int8: %d rows", a.rows);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(ceil_div(a.cols, 128) * split), (unsigned)token_tiles);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    F2S_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, mw, mx, g));
+    return check_launch("linear_int8_tiles_kernel");
+}
+
+// ---- pairs -------------------------------------------------------------------
+
+struct PairArgs {
+    const float* xs;
+    const float* ws;
+    const void* bias;
+    void* y;
+    int64_t ldy;
+    int rows, cols;
+    int bn;          // channels of a tile: 64, 128, 192 or 256
+    int k_blocks, stages;
+    int m_tiles, n_tiles;
+    int boxes;       // y written by TMA
+    uint32_t idesc;
+    int* err;
+};
+
+constexpr int kPairEpilogue = 256;  // 8 warps
+constexpr int kPairThreads = 64 + kPairEpilogue;
+constexpr int kBox = 32 * 128;      // 32 rows of 128 bytes of y
+
+// TMA load by either CTA of a pair, signalling a barrier of the pair's leader.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrive on `bar` in both CTAs of the pair once the MMAs issued so far complete.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            tc::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Bounded wait as tc::mbar_wait_poll, for arrivals from the other CTA too.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
+    for (uint32_t i = 0; i < tc::kSpinLimit; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(tc::smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((i & 63u) == 63u && *reinterpret_cast<volatile int*>(err) != tc::kTcOk) return false;
+    }
+    atomicExch(err, tc::kTcWaitTimeout);
+    return false;
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                         const __grid_constant__ CUtensorMap map_y, const PairArgs g) {
+    constexpr int kBoxCols = 128 / (int)sizeof(T);
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem =
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int S = g.stages;
+    const uint32_t a_bytes = 128 * 128, b_bytes = (uint32_t)g.bn * 64, stage_bytes = a_bytes + b_bytes;
+    unsigned char* boxes = smem + (size_t)S * stage_bytes;                    // 8 warps x kBox
+    float* vectors = reinterpret_cast<float*>(boxes + 8 * kBox);               // 8 warps x [ws 128 | bias 128]
+    uint64_t* full = reinterpret_cast<uint64_t*>(vectors + 8 * 256);          // leader's: both CTAs' bytes
+    uint64_t* empty = full + S;
+    uint64_t* tfull = empty + S;   // [2]
+    uint64_t* tempty = tfull + 2;  // [2] leader's: 16 epilogue warps of both CTAs
+    uint64_t* done = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int tiles = g.m_tiles * g.n_tiles, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
+    // tiles in bands of 8 token tiles, channels outer: the operands of the
+    // tiles that run at one time stay in L2
+    auto tile_at = [&](int t, int& m0, int& n0) {
+        const int per_band = 8 * g.n_tiles, band = t / per_band, r = t - band * per_band;
+        const int high = g.m_tiles - band * 8 < 8 ? g.m_tiles - band * 8 : 8;
+        const int n = r / high;
+        m0 = (band * 8 + r - n * high) * 256;
+        n0 = n * g.bn;
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            tc::mbar_init(&full[s], 1);
+            tc::mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(&tfull[b], 1);
+            tc::mbar_init(&tempty[b], 16);
+        }
+        tc::mbar_init(done, 1);
+        tc::fence_barrier_init();
+        tc::prefetch_tensormap(&map_x);
+        tc::prefetch_tensormap(&map_w);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0, pending = 0, pending_phase = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                int m0, n0;
+                tile_at(t, m0, n0);
+                for (int kb = 0; kb < g.k_blocks; ++kb) {
+                    if (!wait_cluster(&empty[stage], phase ^ 1u, g.err)) {
+                        ok = false;
+                        break;
+                    }
+                    unsigned char* st = smem + (size_t)stage * stage_bytes;
+                    const uint32_t bar = map_rank(tc::smem_u32(&full[stage]), 0);
+                    if (rank == 0) tc::mbar_arrive_expect_tx(&full[stage], 2 * stage_bytes);
+                    tma_load_pair(st, &map_x, bar, kb * kBlockK, m0 + (int)rank * 128);
+                    tma_load_pair(st + a_bytes, &map_w, bar, kb * kBlockK, n0 + (int)rank * (g.bn / 2));
+                    pending |= 1u << stage;
+                    pending_phase = (pending_phase & ~(1u << stage)) | (phase << stage);
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                // let the copies already issued land before the CTAs exit: the
+                // leader's barriers count both CTAs' bytes; a copy of the other
+                // CTA that the leader did not expect any more has a millisecond
+                if (rank == 0)
+                    for (int s = 0; s < S; ++s)
+                        if (pending & (1u << s)) tc::mbar_drain(&full[s], (pending_phase >> s) & 1u);
+                for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int stage = 0, iter = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs, ++iter) {
+                const int buf = iter & 1;
+                if (!wait_cluster(&tempty[buf], ((uint32_t)(iter >> 1) & 1u) ^ 1u, g.err)) break;
+                tc::tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(buf * 256);
+                for (int kb = 0; kb < g.k_blocks; ++kb) {
+                    if (!wait_cluster(&full[stage], phase, g.err)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::tc_fence_after();
+                    const uint32_t st = tc::smem_u32(smem + (size_t)stage * stage_bytes);
+                    const uint64_t a = tc::sw128_desc(st), b = tc::sw128_desc(st + a_bytes);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_i8_pair(d, a + 2 * k, b + 2 * k, g.idesc, (kb | k) ? 1u : 0u);
+                    commit_pair(&empty[stage]);
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (ok) commit_pair(&tfull[buf]);
+            }
+            commit_pair(done);
+            tc::mbar_drain(done, 0);
+        }
+        __syncwarp();
+    } else {
+        const int e = warp - 2;        // 0 .. 7
+        const int quarter = warp & 3;  // TMEM lanes of this warp
+        const int half = e >> 2;       // boxes half, half + 2, ...
+        unsigned char* box = boxes + e * kBox;
+        float* ws = vectors + e * 256;
+        float* bs = ws + 128;
+        int iter = 0;
+        for (int t = pair; t < tiles; t += pairs, ++iter) {
+            int m0, n0;
+            tile_at(t, m0, n0);
+            const int buf = iter & 1;
+            const int row0 = m0 + (int)rank * 128 + quarter * 32, row = row0 + lane;
+            // the scales and biases of this warp's columns (box by box), for
+            // this warp alone: no barrier that another warp could miss
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int l = lane + 32 * i, n = n0 + (half + 2 * (l / kBoxCols)) * kBoxCols + l % kBoxCols;
+                ws[l] = n < g.cols ? __ldg(g.ws + n) : 0.0f;
+                bs[l] = n < g.cols ? bias_at<T>(g.bias, n) : 0.0f;
+            }
+            __syncwarp();
+            const float xs = row < g.rows ? __ldg(g.xs + row) : 0.0f;
+            const bool ok = wait_cluster(&tfull[buf], (uint32_t)(iter >> 1) & 1u, g.err);
+            // a warp that gave up stops with its lanes together
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc::tc_fence_after();
+            const uint32_t acc = tmem + (uint32_t)(buf * 256) + ((uint32_t)(quarter * 32) << 16);
+            int held_at = 0;  // this box's columns in ws, bs
+            for (int c = half * kBoxCols; c < g.bn; c += 2 * kBoxCols, held_at += kBoxCols) {
+                uint32_t packed[32];  // 128 bytes of y: this lane's row of the box
+#pragma unroll
+                for (int p = 0; p < kBoxCols; p += 32) {
+                    uint32_t v[32];
+                    tc::tmem_ld32_issue(acc + c + p, v);
+                    tc::tmem_ld32_wait(v);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 w4 = *reinterpret_cast<const float4*>(ws + held_at + p + j);
+                        const float4 b4 = *reinterpret_cast<const float4*>(bs + held_at + p + j);
+                        const float f0 = fmaf((float)(int)v[j] * xs, w4.x, b4.x);
+                        const float f1 = fmaf((float)(int)v[j + 1] * xs, w4.y, b4.y);
+                        const float f2 = fmaf((float)(int)v[j + 2] * xs, w4.z, b4.z);
+                        const float f3 = fmaf((float)(int)v[j + 3] * xs, w4.w, b4.w);
+                        if constexpr (sizeof(T) == 4) {
+                            packed[j] = __float_as_uint(f0);
+                            packed[j + 1] = __float_as_uint(f1);
+                            packed[j + 2] = __float_as_uint(f2);
+                            packed[j + 3] = __float_as_uint(f3);
+                        } else {
+                            packed[(p + j) / 2] = rows::pack2(f0, f1, T());
+                            packed[(p + j) / 2 + 1] = rows::pack2(f2, f3, T());
+                        }
+                    }
+                }
+                if (c + 2 * kBoxCols >= g.bn) {
+                    // this warp's last read of the accumulator
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_cluster(map_rank(tc::smem_u32(&tempty[buf]), 0));
+                }
+                if (n0 + c >= g.cols) continue;  // past the last column
+                // the previous store has read this box
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                        make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+                if (g.boxes) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                                         reinterpret_cast<uint64_t>(&map_y)),
+                                     "r"(tc::smem_u32(box)), "r"(n0 + c), "r"(row0)
+                                     : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                } else {
+                    // any pitch: the box's rows one by one, lanes along the row
+                    __syncwarp();
+                    const T* held = reinterpret_cast<const T*>(box);
+                    for (int r = 0; r < 32 && row0 + r < g.rows; ++r) {
+                        T* to = static_cast<T*>(g.y) + (int64_t)(row0 + r) * g.ldy + n0 + c;
+#pragma unroll
+                        for (int k = lane; k < kBoxCols; k += 32) {
+                            const int chunk = k * (int)sizeof(T) / 16, in = k % (16 / (int)sizeof(T));
+                            if (n0 + c + k < g.cols)
+                                to[k] = held[(r * 128 + ((chunk ^ (r & 7)) << 4)) / (int)sizeof(T) + in];
+                        }
+                    }
+                }
+            }
+            // a warp without a box in this tile (bn of one box) frees its share too
+            if (half * kBoxCols >= g.bn) {
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_cluster(map_rank(tc::smem_u32(&tempty[buf]), 0));
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+    }
+    // neither CTA leaves, or frees its TMEM, while the other still uses it
+    tc::tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    tc::tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+}
+
+template <typename T>
+int pairs_launch(const Int8Args& a, int bn, cudaStream_t st) {
+    CUtensorMap mx, mw, my;
+    F2S_TRY(operand_map(&mx, a.x, a.ldx, a.rows, a.K, 128));
+    F2S_TRY(operand_map(&mw, a.w, a.ldw, a.cols, a.K, bn / 2));
+    PairArgs g{};
+    g.xs = a.xs;
+    g.ws = a.ws;
+    g.bias = a.bias;
+    g.y = a.y;
+    g.ldy = a.ldy;
+    g.rows = a.rows;
+    g.cols = a.cols;
+    g.bn = bn;
+    g.k_blocks = ceil_div(a.K, kBlockK);
+    g.m_tiles = ceil_div(a.rows, 256);
+    g.n_tiles = ceil_div(a.cols, bn);
+    g.idesc = idesc_i8(256, bn);
+    g.err = tc_error_word();
+    if (!g.err) return fail(F2S_ERR_CUDA, "linear_int8: device error word unavailable");
+    F2S_LIMIT((int64_t)g.m_tiles * g.n_tiles <= INT32_MAX / 2, "linear_int8: %d x %d outputs", a.rows, a.cols);
+    g.boxes = rows::aligned16(a.y) && a.ldy * (int64_t)sizeof(T) % 16 == 0;
+    if (g.boxes)
+        F2S_TRY(make_tensor_map_2d_typed(&my, a.y, sizeof(T) == 4 ? kTmaF32 : kTmaBF16, 128, a.rows, a.cols, a.ldy, 32,
+                                         128 / (int)sizeof(T)));
+    else my = mx;
+    const size_t stage = 128 * 128 + (size_t)bn * 64;
+    const size_t fixed = 1024 + 8 * kBox + 8 * 256 * sizeof(float) + 512;
+    int stages = (int)((kSmemLimit - fixed) / stage);
+    g.stages = stages > 8 ? 8 : stages;
+    const size_t smem = fixed + g.stages * stage;
+    auto kernel = linear_int8_pairs_kernel<T>;
+    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int tiles = g.m_tiles * g.n_tiles, pairs = sm_count() / 2;
+    kernel<<<2 * (tiles < pairs ? tiles : pairs), kPairThreads, smem, st>>>(mx, mw, my, g);
+    return check_launch("linear_int8_pairs_kernel");
+}
+
+}  // namespace
+
+int linear_int8_tiles(const Int8Args& a, cudaStream_t st) {
+    // the token tile that holds the rows, 128 at most; K split until the SMs
+    // each have a CTA, at least two K blocks each
+    const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
+    const int64_t ctas = (int64_t)ceil_div(a.cols, 128) * ceil_div(a.rows, bn);
+    const int k_blocks = ceil_div(a.K, kBlockK);
+    int split = 1;
+    while (split < 8 && ctas * split < sm_count() && k_blocks >= 4 * split) split *= 2;
+    int status = F2S_OK;
+    F2S_DTYPE_SWITCH(a.dtype, switch (bn) {
+        case 16: status = tiles_launch<T, 16>(a, split, st); break;
+        case 32: status = tiles_launch<T, 32>(a, split, st); break;
+        case 64: status = tiles_launch<T, 64>(a, split, st); break;
+        default: status = tiles_launch<T, 128>(a, split, st); break;
+    });
+    return status;
+}
+
+int linear_int8_pairs(const Int8Args& a, cudaStream_t st) {
+    // the channel tile with the fewest columns computed (one of 64 takes as
+    // long as one of 128), the larger on ties
+    int bn = 256;
+    for (int c : {192, 128, 64})
+        if (ceil_div(a.cols, c) * (c < 128 ? 128 : c) < ceil_div(a.cols, bn) * bn) bn = c;
+    int status = F2S_OK;
+    F2S_DTYPE_SWITCH(a.dtype, status = pairs_launch<T>(a, bn, st));
+    return status;
+}
+
+}  // namespace f2s

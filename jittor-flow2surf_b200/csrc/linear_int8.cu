@@ -1,7 +1,7 @@
 // Product of 8-bit integer rows with scales for each token and channel:
 //   y[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k] + b[n],
 // the sum exact in 32 bits (K <= 131,071 keeps 2^14 K below 2^31).
-#include "kernels.cuh"
+#include "gemm_int8.cuh"
 #include "row_ops.cuh"
 
 namespace f2s {
@@ -10,19 +10,6 @@ namespace {
 using namespace rows;
 
 constexpr int kMaxK = 131071;
-
-struct Int8Args {
-    const int8_t* x;
-    int64_t ldx;
-    const float* xs;
-    const int8_t* w;
-    int64_t ldw;
-    const float* ws;
-    const void* bias;  // of y's type, or null
-    void* y;
-    int64_t ldy;
-    int rows, cols, K;
-};
 
 // Any pitch and alignment: 64 x 64 outputs per block of 256 threads, 4 x 4
 // each, K in steps of 64 staged in shared memory as words of four, four
@@ -90,9 +77,12 @@ extern "C" int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scal
     if (rows == 0) return F2S_OK;
     F2S_REQUIRE(x && x_scale && w && w_scale && y, "linear_int8: null pointer");
     F2S_REQUIRE(ldx >= K && ldw >= K && ldy >= cols, "linear_int8: row pitch below the row");
-    f2s::Int8Args g{x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, rows, cols, K};
+    f2s::Int8Args g{x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, dtype, rows, cols, K};
     cudaStream_t st = f2s::as_stream(stream);
     f2s::TraceScope trace(f2s::kTagGemmInt8, st);
+    using f2s::rows::aligned16;
+    if (aligned16(x) && aligned16(w) && (ldx % 16 == 0 || rows == 1) && (ldw % 16 == 0 || cols == 1))
+        return rows >= 1024 ? f2s::linear_int8_pairs(g, st) : f2s::linear_int8_tiles(g, st);
     int status = F2S_OK;
     F2S_DTYPE_SWITCH(dtype, status = f2s::any_launch<T>(g, st));
     return status;

@@ -311,11 +311,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
     }
 
 // The three element types of these operators (f2s_dtype).
-#define F2S_DTYPE_SWITCH(dtype, BODY)                             \
-    switch (dtype) {                                              \
-        case F2S_DTYPE_F32: { using T = float; BODY; break; }            \
-        case F2S_DTYPE_BF16: { using T = __nv_bfloat16; BODY; break; }   \
-        default: { using T = __half; BODY; break; }                \
+#define F2S_DTYPE_SWITCH(dtype, ...)                                     \
+    switch (dtype) {                                                     \
+        case F2S_DTYPE_F32: { using T = float; __VA_ARGS__; break; }          \
+        case F2S_DTYPE_BF16: { using T = __nv_bfloat16; __VA_ARGS__; break; } \
+        default: { using T = __half; __VA_ARGS__; break; }                    \
     }
 
 inline int check_dtype(const char* what, int dtype) {

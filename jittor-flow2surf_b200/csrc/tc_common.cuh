@@ -439,8 +439,8 @@ __host__ __device__ constexpr uint32_t make_idesc(int M, int N, uint32_t ab_form
 int make_tensor_map_2d(CUtensorMap* map, const void* base, bool fp32, int64_t rows,
                        int64_t cols, int64_t ld, int box_rows, int box_cols);
 
-// Element types of the typed form: fp32, bf16, fp16.
-enum TmaType : int { kTmaF32 = 0, kTmaBF16 = 1, kTmaF16 = 2 };
+// Element types of the typed form: fp32, bf16, fp16, bytes.
+enum TmaType : int { kTmaF32 = 0, kTmaBF16 = 1, kTmaF16 = 2, kTmaU8 = 3 };
 // The same with an explicit element type and swizzle span (128 or 64 bytes).
 int make_tensor_map_2d_typed(CUtensorMap* map, const void* base, TmaType type, int swizzle_bytes,
                              int64_t rows, int64_t cols, int64_t ld, int box_rows, int box_cols);

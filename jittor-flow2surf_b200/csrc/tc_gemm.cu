@@ -819,7 +819,7 @@ int make_tensor_map_2d_typed(CUtensorMap* map, const void* base, TmaType type, i
                              int64_t rows, int64_t cols, int64_t ld, int box_rows, int box_cols) {
     EncodeTiledFn enc = encode_fn();
     if (!enc) return fail(F2S_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-    const int64_t elem = type == kTmaF32 ? 4 : 2;
+    const int64_t elem = type == kTmaF32 ? 4 : type == kTmaU8 ? 1 : 2;
     F2S_REQUIRE(((uintptr_t)base & 15) == 0, "tensor map base must be 16-byte aligned");
     F2S_REQUIRE((ld * elem) % 16 == 0, "tensor map row pitch must be a multiple of 16 bytes");
     F2S_REQUIRE(swizzle_bytes == 128 || swizzle_bytes == 64, "tensor map swizzle %d", swizzle_bytes);
@@ -830,6 +830,7 @@ int make_tensor_map_2d_typed(CUtensorMap* map, const void* base, TmaType type, i
     const cuuint32_t estr[2] = {1, 1};
     const CUtensorMapDataType dt = type == kTmaF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : type == kTmaBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : type == kTmaU8   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE,
