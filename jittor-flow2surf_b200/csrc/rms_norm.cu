@@ -43,11 +43,11 @@ __device__ __forceinline__ float reciprocal_rms(float sum, int C, float eps) {
 // k8: 8-bit rows. The products s w of a 16-bit type are exact in fp32; those of
 // fp32 are taken in 64 bits for the maximum and at rounding borders.
 template <typename T, int E, int TPR, bool kWide, bool k8>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR)
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, 2 * sizeof(T)))
 add_rms_norm_kernel(const NormArgs g) {
     using S = Slice<T, E, TPR, kWide>;
     constexpr bool kExact64 = k8 && sizeof(T) == 4;
-    using M = typename std::conditional<kExact64, unsigned long long, uint32_t>::type;
+    using M = typename std::conditional<kExact64, unsigned long long, float>::type;
     __shared__ M shared_m[32];
     __shared__ float shared_a[32];
     const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
@@ -55,59 +55,88 @@ add_rms_norm_kernel(const NormArgs g) {
     // rows past the end take part in the shuffles and write nothing
     const bool live = row < g.nrows;
     const int C = live ? g.C : 0;
-    float s[E], w[E];
-    S::load(static_cast<const T*>(g.x) + (live ? row : 0) * g.ldx, C, t, s);
+    const int64_t at = live ? row : 0;
+    const T* weight = static_cast<const T*>(g.weight);
+    const T* from = static_cast<const T*>(g.x) + at * g.ldx;
+    Held<T, E, kWide> s, w;
+    load_held<S>(from, C, t, s);
     if (g.residual) {
-        float r[E];
-        S::load(static_cast<const T*>(g.residual) + (live ? row : 0) * g.ldr, C, t, r);
-        S::load(static_cast<const T*>(g.weight), C, t, w);
+        Held<T, E, kWide> r;
+        load_held<S>(static_cast<const T*>(g.residual) + at * g.ldr, C, t, r);
+        load_held<S>(weight, C, t, w);
 #pragma unroll
-        for (int i = 0; i < E; ++i) s[i] = rounded<T>(s[i] + r[i]);
-        S::store(static_cast<T*>(g.stream) + (live ? row : 0) * (int64_t)g.C, C, t, s);
+        for (int i = 0; i < E; i += 8) {
+            float a[8], b[8];
+            s.get(i, a);
+            r.get(i, b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] += b[j];
+            s.set(i, a);
+        }
+        T* to = static_cast<T*>(g.stream) + at * (int64_t)g.C;
+        store_held<S>(to, C, t, s);
+        from = to;
     } else {
-        S::load(static_cast<const T*>(g.weight), C, t, w);
+        load_held<S>(weight, C, t, w);
     }
     float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) sum = fmaf(s[i], s[i], sum);
     M m = 0;
-    if constexpr (k8) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            M b;
-            if constexpr (kExact64)
-                b = (unsigned long long)__double_as_longlong(fabs((double)s[i] * (double)w[i]));
-            else b = abs_bits(s[i] * w[i]);
-            m = b > m ? b : m;
+    for (int i = 0; i < E; i += 8) {
+        float a[8], b[8];
+        s.get(i, a);
+        w.get(i, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sum = fmaf(a[j], a[j], sum);
+            if constexpr (kExact64) {
+                const M p = (M)__double_as_longlong(fabs((double)a[j] * (double)b[j]));
+                m = p > m ? p : m;
+            } else if constexpr (k8) {
+                b[j] *= a[j];
+            }
         }
+        if constexpr (k8 && !kExact64) m = max_abs(b, m);
     }
-    row_sum_max<TPR>(sum, m, shared_m, shared_a);
+    row_sum_max<TPR, true, k8>(sum, m, shared_a, shared_m);
     const float rstd = reciprocal_rms(sum, g.C, g.eps);
     if constexpr (k8) {
-        double largest;
-        bool finite;
-        if constexpr (kExact64) {
-            largest = __longlong_as_double((long long)m);
-            finite = m < kInfBits64 && largest < 3.0e38;
-        } else {
-            largest = (double)__uint_as_float(m);
-            finite = m < kInfBits;
-        }
-        const float lf = (float)largest;
-        const float inv = 127.0f / lf;
-        float p[E];
+        using L = typename std::conditional<kExact64, double, float>::type;
+        L largest;
+        if constexpr (kExact64) largest = __longlong_as_double((long long)m);
+        else largest = m;
+        const Rounding<L> rounding(largest);
 #pragma unroll
-        for (int i = 0; i < E; ++i) p[i] = s[i] * w[i];
-        uint32_t q[E];
-        round8_row(p, inv, finite ? largest : 0.0, finite && lf >= kTiny, q,
-                   [&](int i) { return (double)s[i] * (double)w[i]; });
-        S::store8(g.q + (live ? row : 0) * g.ldq, C, t, q);
+        for (int i = 0; i < E; i += 8) {
+            float a[8], b[8];
+            s.get(i, a);
+            w.get(i, b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] *= b[j];
+            if constexpr (kExact64) {
+                // `from` holds the stream: x, or this thread's own channels of it
+                store8_chunk<S, kWide>(g.q + at * g.ldq, C, t, i, a, rounding, [&](int j) {
+                    const int c = S::channel(i + j, t);
+                    return c < C ? (double)from[c] * (double)weight[c] * (double)rounding.scale : 0.0;
+                });
+            } else {
+                store8_chunk<S, kWide>(g.q + at * g.ldq, C, t, i, a, rounding, [&](int j) { return a[j]; });
+            }
+        }
         if (live && t == 0)
-            g.scale[row] = finite ? (float)(largest / 127.0 * (double)rstd) : __int_as_float(0x7fc00000);
+            g.scale[row] = (float)largest < kInf ? (float)((double)largest / 127.0 * (double)rstd)
+                                                 : __int_as_float(0x7fc00000);
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) s[i] = s[i] * rstd * w[i];
-        S::store(static_cast<T*>(g.y) + (live ? row : 0) * (int64_t)g.C, C, t, s);
+        for (int i = 0; i < E; i += 8) {
+            float a[8], b[8];
+            s.get(i, a);
+            w.get(i, b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] = a[j] * rstd * b[j];
+            s.set(i, a);
+        }
+        store_held<S>(static_cast<T*>(g.y) + at * (int64_t)g.C, C, t, s);
     }
 }
 
@@ -117,14 +146,14 @@ int norm_launch(const NormArgs& g, int dtype, cudaStream_t st) {
     const bool wide = g.C % vec == 0 && aligned16(g.x) && (g.ldx % vec == 0 || g.nrows == 1) && aligned16(g.weight) &&
                       (!g.residual || (aligned16(g.residual) && (g.ldr % vec == 0 || g.nrows == 1) && aligned16(g.stream))) &&
                       (k8 ? (aligned16(g.q) && (g.ldq % vec == 0 || g.nrows == 1)) : aligned16(g.y));
-    const Shape s = pick_shape(g.nrows, g.C, wide);
+    const Shape s = pick_shape(kForward, size, g.nrows, g.C, wide);
     const int64_t blocks = ceil_div64(g.nrows, block_rows(s.tpr));
     F2S_LIMIT(blocks <= INT32_MAX, "add_rms_norm: %lld rows", (long long)g.nrows);
     TraceScope trace(kTagRmsNorm, st);
-#define F2S_LAUNCH(T, E, TPR, W) \
-    add_rms_norm_kernel<T, E, TPR, W, k8><<<(unsigned)blocks, block_threads(TPR), 0, st>>>(g)
-    F2S_DTYPE_SWITCH(dtype, F2S_ROW_DISPATCH(s, wide, T, F2S_LAUNCH));
-#undef F2S_LAUNCH
+    F2S_DTYPE_SWITCH(dtype, dispatch<kForward, sizeof(T)>(s, wide, [&](auto e, auto tpr, auto w) {
+        add_rms_norm_kernel<T, e.value, tpr.value, w.value, k8>
+            <<<(unsigned)blocks, block_threads(tpr.value), 0, st>>>(g);
+    }));
     return check_launch("add_rms_norm_kernel");
 }
 
@@ -150,8 +179,15 @@ struct NormGradArgs {
     float* partial;  // (blocks, C), or null: no weight gradient
 };
 
+// Blocks per SM: 1,024 threads with 8 16-bit channels each (64 registers), 512
+// with more (128).
+constexpr int grad_resident(int tpr, int E, int size) {
+    const int threads = E * size <= 16 ? 1024 : 512;
+    return threads / block_threads(tpr) > 0 ? threads / block_threads(tpr) : 1;
+}
+
 template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR)
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, grad_resident(TPR, E, sizeof(T)))
 add_rms_norm_grad_kernel(const NormGradArgs g) {
     using S = Slice<T, E, TPR, kWide>;
     constexpr int kRows = TPR <= 32 ? 256 / TPR : 1;
@@ -161,29 +197,48 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
     float dw[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) dw[i] = 0.0f;
+    // Rows of one warp or less: the other warps' loads hide a row's latency.
+    // Rows of a block: its warps wait for one another, so the next row is on
+    // its way meanwhile.
+    constexpr bool kAhead = TPR > 32;
+    Held<T, E, kWide> w, s, dy, ds, s_next, dy_next, ds_next;
+    load_held<S>(static_cast<const T*>(g.weight), g.C, t, w);
+    auto fetch = [&](int64_t row) {
+        const bool in = row < g.nrows;
+        const int64_t at = in ? row : 0;
+        const int C = in ? g.C : 0;
+        load_held<S>(static_cast<const T*>(g.s) + at * g.lds, C, t, s_next);
+        load_held<S>(static_cast<const T*>(g.dy) + at * g.lddy, C, t, dy_next);
+        if (g.ds) load_held<S>(static_cast<const T*>(g.ds) + at * g.ldds, C, t, ds_next);
+    };
+    const int64_t stride = (int64_t)gridDim.x * kRows;
+    if constexpr (kAhead) fetch(blockIdx.x);
     int parity = 0;
-    for (int64_t first = (int64_t)blockIdx.x * kRows; first < g.nrows; first += (int64_t)gridDim.x * kRows) {
+    for (int64_t first = (int64_t)blockIdx.x * kRows; first < g.nrows; first += stride) {
         const int64_t row = first + group;
         const bool live = row < g.nrows;
         const int64_t at = live ? row : 0;
         const int C = live ? g.C : 0;
-        float s[E], dy[E], w[E];
-        S::load(static_cast<const T*>(g.s) + at * g.lds, C, t, s);
-        S::load(static_cast<const T*>(g.dy) + at * g.lddy, C, t, dy);
-        S::load(static_cast<const T*>(g.weight), C, t, w);
+        if constexpr (!kAhead) fetch(row);
+        s = s_next;
+        dy = dy_next;
+        ds = ds_next;
+        if constexpr (kAhead) fetch(row + stride);
         float sum = 0.0f, along = 0.0f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            sum = fmaf(s[i], s[i], sum);
-            w[i] *= dy[i];
-            along = fmaf(w[i], s[i], along);
-        }
-        constexpr int kWidth = TPR < 32 ? TPR : 32;
+        for (int i = 0; i < E; i += 8) {
+            float a[8], b[8], c[8];
+            s.get(i, a);
+            dy.get(i, b);
+            w.get(i, c);
 #pragma unroll
-        for (int o = kWidth / 2; o > 0; o >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            along += __shfl_xor_sync(0xffffffffu, along, o);
+            for (int j = 0; j < 8; ++j) {
+                sum = fmaf(a[j], a[j], sum);
+                along = fmaf(b[j] * c[j], a[j], along);
+            }
         }
+        sum = lanes_sum<TPR>(sum);
+        along = lanes_sum<TPR>(along);
         if constexpr (TPR > 32) {
             // two buffers by turns: a row's partial sums are read before the
             // barrier of the next row, and overwritten only after it
@@ -194,33 +249,30 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
                 shared_b[parity][warp] = along;
             }
             __syncthreads();
-            sum = lane < kWarps ? shared_a[parity][lane] : 0.0f;
-            along = lane < kWarps ? shared_b[parity][lane] : 0.0f;
-#pragma unroll
-            for (int o = kWarps / 2; o > 0; o >>= 1) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                along += __shfl_xor_sync(0xffffffffu, along, o);
-            }
-            sum = __shfl_sync(0xffffffffu, sum, 0);
-            along = __shfl_sync(0xffffffffu, along, 0);
+            sum = lanes_sum<kWarps>(shared_a[parity][lane % kWarps]);
+            along = lanes_sum<kWarps>(shared_b[parity][lane % kWarps]);
             parity ^= 1;
         }
         // 0 past the last row: with eps = 0 its reciprocal would put NaN into dw
         const float rstd = live ? reciprocal_rms(sum, g.C, g.eps) : 0.0f;
         const float mean = along * rstd / (float)g.C;  // mean(u n)
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float n = s[i] * rstd;
-            dw[i] = fmaf(dy[i], n, dw[i]);
-            s[i] = rstd * (w[i] - n * mean);
-        }
-        if (g.ds) {
-            float ds[E];
-            S::load(static_cast<const T*>(g.ds) + at * g.ldds, C, t, ds);
+        for (int i = 0; i < E; i += 8) {
+            float a[8], b[8], c[8], d[8];
+            s.get(i, a);
+            dy.get(i, b);
+            w.get(i, c);
+            if (g.ds) ds.get(i, d);
 #pragma unroll
-            for (int i = 0; i < E; ++i) s[i] += ds[i];
+            for (int j = 0; j < 8; ++j) {
+                const float n = a[j] * rstd;
+                dw[i + j] = fmaf(b[j], n, dw[i + j]);
+                a[j] = rstd * (b[j] * c[j] - n * mean);
+                if (g.ds) a[j] += d[j];
+            }
+            s.set(i, a);
         }
-        S::store(static_cast<T*>(g.dx) + at * (int64_t)g.C, C, t, s);
+        store_held<S>(static_cast<T*>(g.dx) + at * (int64_t)g.C, C, t, s);
     }
     if (!g.partial) return;
     float* mine = g.partial + (int64_t)blockIdx.x * g.C;
@@ -254,39 +306,49 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
     }
 }
 
-// dw[c] = sum over blocks of partial[block][c]: 32 channels x 8 slices of the
-// blocks per CTA.
+// dw[c] = sum over blocks of partial[block][c]: 32 channels x 32 slices of the
+// blocks per CTA, four loads of a slice in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) weight_grad_kernel(const float* __restrict__ partial, int blocks, int C,
-                                                          T* __restrict__ dw) {
-    __shared__ float sums[8][32];
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int blocks, int C,
+                                                           T* __restrict__ dw) {
+    __shared__ float sums[32][33];
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float a = 0.0f;
-    if (c < C)
-        for (int b = slice; b < blocks; b += 8) a += partial[(int64_t)b * C + c];
+    if (c < C) {
+#pragma unroll 4
+        for (int b = slice; b < blocks; b += 32) a += partial[(int64_t)b * C + c];
+    }
     sums[slice][lane] = a;
     __syncthreads();
-    if (slice == 0 && c < C) {
-#pragma unroll
-        for (int k = 1; k < 8; ++k) a += sums[k][lane];
-        dw[c] = from_f32<T>(a);
-    }
+    // warp `slice` sums the slices of channel `slice`
+    a = f2s_warp_sum(sums[lane][slice]);
+    const int at = blockIdx.x * 32 + slice;
+    if (lane == 0 && at < C) dw[at] = from_f32<T>(a);
 }
 
 template <typename T>
 void weight_grad_launch(const float* partial, int blocks, int C, void* dw, cudaStream_t st) {
-    weight_grad_kernel<T><<<ceil_div(C, 32), 256, 0, st>>>(partial, blocks, C, static_cast<T*>(dw));
+    weight_grad_kernel<T><<<ceil_div(C, 32), 1024, 0, st>>>(partial, blocks, C, static_cast<T*>(dw));
 }
 
-// Blocks of the backward: enough to fill the SMs, each with several rows to
-// share its dw over.
-int grad_blocks(int64_t nrows, int C) {
-    const Shape s = pick_shape(nrows, C, true);
+// Blocks of the backward: those that are resident at one time, each with
+// several rows to share its dw over.
+int grad_blocks(int64_t nrows, const Shape& s, int dtype) {
     const int64_t all = ceil_div64(nrows, block_rows(s.tpr));
-    const int per_sm = s.tpr <= 32 ? 4 : s.tpr == 128 ? 8 : 2;
-    const int64_t most = (int64_t)sm_count() * per_sm;
+    const int64_t most = (int64_t)sm_count() * grad_resident(s.tpr, s.e, dtype_size(dtype));
     return (int)(all < most ? all : most);
+}
+
+// Enough for any type and layout of (nrows, C): the most blocks of its shapes.
+size_t grad_workspace(int64_t nrows, int C) {
+    int blocks = 0;
+    for (int dtype : {F2S_DTYPE_F32, F2S_DTYPE_BF16})
+        for (bool wide : {false, true}) {
+            const int b = grad_blocks(nrows, pick_shape(kGrad, dtype_size(dtype), nrows, C, wide), dtype);
+            blocks = b > blocks ? b : blocks;
+        }
+    return (size_t)blocks * C * sizeof(float);
 }
 
 int check_norm(const char* what, int dtype, int64_t nrows, int C, float eps) {
@@ -324,7 +386,7 @@ extern "C" int f2s_add_rms_norm_int8(const void* x, int64_t ldx, const void* res
 extern "C" int f2s_add_rms_norm_backward_workspace_bytes(int64_t rows, int C, size_t* bytes) {
     F2S_TRY(f2s::check_norm("add_rms_norm_backward", F2S_DTYPE_F32, rows, C, 0.0f));
     F2S_REQUIRE(bytes, "add_rms_norm_backward: null pointer");
-    *bytes = (size_t)f2s::grad_blocks(rows, C) * C * sizeof(float);
+    *bytes = f2s::grad_workspace(rows, C);
     return F2S_OK;
 }
 
@@ -342,21 +404,21 @@ extern "C" int f2s_add_rms_norm_backward(const void* s, int64_t lds, const void*
     }
     F2S_REQUIRE(s && weight && dy && dx, "add_rms_norm_backward: null pointer");
     F2S_REQUIRE(lds >= C && lddy >= C && (!ds || ldds >= C), "add_rms_norm_backward: row pitch below C=%d", C);
-    const int blocks = grad_blocks(rows, C);
-    if (dweight && (!workspace || workspace_bytes < (size_t)blocks * C * sizeof(float)))
+    const size_t needed = grad_workspace(rows, C);
+    if (dweight && (!workspace || workspace_bytes < needed))
         return fail(F2S_ERR_WORKSPACE, "add_rms_norm_backward: workspace of %zu bytes, %zu needed", workspace_bytes,
-                    (size_t)blocks * C * sizeof(float));
+                    needed);
     const int vec = 16 / dtype_size(dtype);
     auto pitched = [&](const void* p, int64_t ld) { return aligned16(p) && (ld % vec == 0 || rows == 1); };
     const bool wide = C % vec == 0 && pitched(s, lds) && pitched(dy, lddy) && (!ds || pitched(ds, ldds)) &&
                       aligned16(weight) && aligned16(dx);
     NormGradArgs g{s, lds, weight, dy, lddy, ds, ldds, rows, C, eps, dx, dweight ? static_cast<float*>(workspace) : nullptr};
-    const Shape shape = pick_shape(rows, C, wide);
+    const Shape shape = pick_shape(kGrad, dtype_size(dtype), rows, C, wide);
+    const int blocks = grad_blocks(rows, shape, dtype);
     TraceScope trace(kTagRmsNorm, st);
-#define F2S_LAUNCH(T, E, TPR, W) \
-    add_rms_norm_grad_kernel<T, E, TPR, W><<<blocks, block_threads(TPR), 0, st>>>(g)
-    F2S_DTYPE_SWITCH(dtype, F2S_ROW_DISPATCH(shape, wide, T, F2S_LAUNCH));
-#undef F2S_LAUNCH
+    F2S_DTYPE_SWITCH(dtype, dispatch<kGrad, sizeof(T)>(shape, wide, [&](auto e, auto tpr, auto w) {
+        add_rms_norm_grad_kernel<T, e.value, tpr.value, w.value><<<blocks, block_threads(tpr.value), 0, st>>>(g);
+    }));
     F2S_TRY(check_launch("add_rms_norm_grad_kernel"));
     if (!dweight) return F2S_OK;
     F2S_DTYPE_SWITCH(dtype, weight_grad_launch<T>(static_cast<const float*>(workspace), blocks, C, dweight, st));

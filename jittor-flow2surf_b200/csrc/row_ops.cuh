@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace f2s {
@@ -118,126 +120,259 @@ struct Slice {
             else row[c] = from_f32<T>(v[i]);
         }
     }
+};
 
-    // low bytes of q[i]; `row` 8-byte aligned where kWide (a multiple of 16 in fact)
-    __device__ static __forceinline__ void store8(int8_t* row, int C, int t, const uint32_t (&q)[E]) {
+// A thread's E channels as they are stored: packed pairs of a 16-bit type read
+// in vectors (half the registers of fp32 values), fp32 otherwise. Used in
+// chunks of 8.
+template <typename T, int E, bool kWide>
+struct Held {
+    static constexpr bool kPacked = kWide && sizeof(T) == 2;
+    static_assert(E % 8 == 0, "whole chunks");
+    uint4 u[kPacked ? E / 8 : 1];
+    float f[kPacked ? 1 : E];
+
+    __device__ __forceinline__ void get(int i, float (&v)[8]) const {
+        if constexpr (kPacked) {
+            unpack16<T>(u[i / 8], v);
+        } else {
 #pragma unroll
-        for (int i = 0; i < E; i += V) {
-            const int c = channel(i, t);
-            if (c >= C) continue;
-            if constexpr (kWide) {
-                uint32_t w[V / 4];
+            for (int j = 0; j < 8; ++j) v[j] = f[i + j];
+        }
+    }
+    // Values rounded to T.
+    __device__ __forceinline__ void set(int i, const float (&v)[8]) {
+        if constexpr (kPacked) {
+            u[i / 8] = pack16<T>(v);
+        } else {
 #pragma unroll
-                for (int j = 0; j < V / 4; ++j)
-                    w[j] = __byte_perm(__byte_perm(q[i + 4 * j], q[i + 4 * j + 1], 0x0040),
-                                       __byte_perm(q[i + 4 * j + 2], q[i + 4 * j + 3], 0x0040), 0x5410);
-                if constexpr (V == 8) *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t*>(row + c) = w[0];
-            } else {
-                row[c] = (int8_t)(q[i] & 0xffu);
-            }
+            for (int j = 0; j < 8; ++j) f[i + j] = to_f32<T>(from_f32<T>(v[j]));
         }
     }
 };
 
-// v rounded to T and back: what a row stored in T holds.
-template <typename T>
-__device__ __forceinline__ float rounded(float v) {
-    return to_f32<T>(from_f32<T>(v));
+template <typename S, typename T, int E, bool kWide>
+__device__ __forceinline__ void load_held(const T* row, int C, int t, Held<T, E, kWide>& h) {
+    if constexpr (Held<T, E, kWide>::kPacked) {
+#pragma unroll
+        for (int i = 0; i < E; i += 8) {
+            const int c = S::channel(i, t);
+            h.u[i / 8] = c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+        }
+    } else {
+        S::load(row, C, t, h.f);
+    }
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-constexpr uint32_t kInfBits = 0x7f800000u;
-constexpr unsigned long long kInfBits64 = 0x7ff0000000000000ull;
-
-// Sum of `a` (fp32) and maximum of `m` over the TPR threads of a row; every
-// thread gets both. Magnitudes are compared as bit patterns, so that infinity
-// and NaN, whose patterns lie above every finite value's, are not lost as in
-// a floating-point maximum. `shared` holds 2 * TPR / 32 entries for TPR > 32;
-// two uses need a barrier between them.
-template <int TPR, typename M>
-__device__ __forceinline__ void row_sum_max(float& a, M& m, M* shared_m, float* shared_a) {
-    constexpr int kWidth = TPR < 32 ? TPR : 32;
+template <typename S, typename T, int E, bool kWide>
+__device__ __forceinline__ void store_held(T* row, int C, int t, const Held<T, E, kWide>& h) {
+    if constexpr (Held<T, E, kWide>::kPacked) {
 #pragma unroll
-    for (int o = kWidth / 2; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        const M other = __shfl_xor_sync(0xffffffffu, m, o);
+        for (int i = 0; i < E; i += 8) {
+            const int c = S::channel(i, t);
+            if (c < C) *reinterpret_cast<uint4*>(row + c) = h.u[i / 8];
+        }
+    } else {
+        S::store(row, C, t, h.f);
+    }
+}
+
+constexpr float kInf = __builtin_huge_valf();
+
+// Largest of a and the magnitudes of b and c, keeping a NaN (fmaxf drops it), so
+// that a row's largest magnitude tells whether all of the row is finite.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_abs(const float (&v)[8], float m) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) m = max_abs(m, v[j], v[j + 1]);
+    return m;
+}
+
+template <int TPR>
+__device__ __forceinline__ float lanes_max(float m) {
+    if constexpr (TPR >= 32) {
+        float r;
+        asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(m));
+        return r;
+    } else {
+#pragma unroll
+        for (int o = TPR / 2; o > 0; o >>= 1) m = max_abs(m, m, __shfl_xor_sync(0xffffffffu, m, o));
+        return m;
+    }
+}
+// In 64 bits, on the bit patterns of magnitudes: infinity's and NaN's lie above
+// every finite value's.
+template <int TPR>
+__device__ __forceinline__ unsigned long long lanes_max(unsigned long long m) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, m, o);
         m = other > m ? other : m;
     }
+    return m;
+}
+template <int TPR>
+__device__ __forceinline__ float lanes_sum(float a) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    return a;
+}
+
+// Sum of `a` (kSum) and maximum of `m` (kMax) over the TPR threads of a row;
+// every thread gets both. The shared arrays hold TPR / 32 entries for TPR > 32;
+// two uses need a barrier between them.
+template <int TPR, bool kSum, bool kMax, typename M>
+__device__ __forceinline__ void row_sum_max(float& a, M& m, float* shared_a, M* shared_m) {
+    if constexpr (kSum) a = lanes_sum<TPR>(a);
+    if constexpr (kMax) m = lanes_max<TPR>(m);
     if constexpr (TPR > 32) {
         constexpr int kWarps = TPR / 32;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         if (lane == 0) {
-            shared_a[warp] = a;
-            shared_m[warp] = m;
+            if constexpr (kSum) shared_a[warp] = a;
+            if constexpr (kMax) shared_m[warp] = m;
         }
         __syncthreads();
-        a = lane < kWarps ? shared_a[lane] : 0.0f;
-        m = lane < kWarps ? shared_m[lane] : M(0);
-#pragma unroll
-        for (int o = kWarps / 2; o > 0; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            const M other = __shfl_xor_sync(0xffffffffu, m, o);
-            m = other > m ? other : m;
-        }
-        a = __shfl_sync(0xffffffffu, a, 0);
-        m = __shfl_sync(0xffffffffu, m, 0);
+        // each lane one of the warps' values, some twice
+        if constexpr (kSum) a = lanes_sum<kWarps>(shared_a[lane % kWarps]);
+        if constexpr (kMax) m = lanes_max<kWarps>(shared_m[lane % kWarps]);
     }
 }
 
 // ---- rounding to 8 bits ----------------------------------------------------
 // q = the whole number nearest to 127 v / m (m the row's largest magnitude),
 // the even one at a tie, of the exact quotient. In fp32, t = v inv with
-// inv = 127 / m is off by at most 127 (2^-24 of inv, 2^-24 of a rounded v) =
-// 1.6e-5, so the nearest whole number of t is the answer unless t lies within
-// kBorder of a half; there (about one value in 15,000) the halves are compared
-// in 64 bits, where 254 v and (2 k + 1) m are exact (v of 48 bits: to 2^-53).
+// inv = 127 / m is off by at most 127 (2^-23 + 2^-24 of inv, 2^-24 of a rounded
+// v, 2^-24 of a rounded m) = 3.8e-5, so the nearest whole number of t is the
+// answer unless t lies next to a half, past kBorder. There the sign of
+// 254 v - c m with c / 2 that half decides, taken without rounding. (One value in
+// 10,000, but more where v and m have few bits: the quotients of bf16 values
+// are exact halves about once in 1,000.)
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
-constexpr float kBorder = 0.49997f;
-// below this m the fp32 quotient may overflow or lose bits: all in 64 bits
-constexpr float kTiny = 1e-30f;
+constexpr float kBorder = 0.49995f;
+// Below 1e-30, 127 / m may overflow and products lose bits, and above 1e30
+// 254 v may overflow: such a row is scaled by 2^80 or 2^-80 first, which changes
+// no quotient (what falls below the smallest number is far below a half).
+constexpr float kTiny = 1e-30f, kHuge = 1e30f;
+constexpr float kScaleTiny = 0x1p80f, kScaleHuge = 0x1p-80f;
 
-static __device__ __noinline__ uint32_t round8_exact(double v, double m) {
-    double k = floor(127.0 * v / m);
-    const double twice = 254.0 * v - (2.0 * k + 1.0) * m;
-    // k is the floor up to its own rounding next to a whole number, where
-    // both neighbours' halves are far
-    if (twice > 0.0 || (twice == 0.0 && ((int)k & 1))) k += 1.0;
-    k = k > 127.0 ? 127.0 : k < -127.0 ? -127.0 : k;
-    return (uint32_t)(int)k;
+// 254 v - c m of fp32 values, c odd and below 256 in magnitude: each product is
+// the sum of its rounding and an error of at most 8 bits; the two are within
+// 2^-10 of each other, so their differences are exact and the sign is right.
+__device__ __forceinline__ float half_side(float v, float m, float c) {
+    const float p = __fmul_rn(254.0f, v), q = __fmul_rn(c, m);
+    return __fadd_rn(__fsub_rn(p, q), __fsub_rn(__fmaf_rn(254.0f, v, -p), __fmaf_rn(c, m, -q)));
+}
+// The same of a product v = s w of fp32 values and a 64-bit m: v has 48 bits and
+// 254 v 56, of which 53 are kept.
+__device__ __forceinline__ float half_side(double v, double m, float c) {
+    return (float)(254.0 * v - (double)c * m);
 }
 
-// t's nearest whole number in the low bits; `off` grows to the largest
-// distance of a t from it.
-__device__ __forceinline__ uint32_t round8(float v, float inv, float& off) {
-    const float shifted = __fmaf_rn(v, inv, kMagic);
-    const float whole = __fsub_rn(shifted, kMagic);
-    off = fmaxf(off, fabsf(__fmaf_rn(v, inv, -whole)));
-    return __float_as_uint(shifted);
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// E values of one thread to 8 bits, v the fp32 values and at(i) the exact
-// ones. `fast`: m is finite and at least kTiny; otherwise m is zero or not
-// finite (all zero bits), or tiny (all exact).
-template <int E, typename F>
-__device__ __forceinline__ void round8_row(const float (&v)[E], float inv, double m, bool fast,
-                                           uint32_t (&q)[E], F at) {
-    if (fast) {
-        float off = 0.0f;
+// How a row of largest magnitude m is rounded.
+template <typename M>
+struct Rounding {
+    M m;          // scaled
+    float inv;    // 127 / m
+    float scale;  // of the row's values, 1 unless `odd`
+    bool odd;     // a tiny, huge, zero or not finite row
+    bool zero;    // a row of zeros, or one that is not finite
+    __device__ __forceinline__ explicit Rounding(M largest) : m(largest), scale(1.0f) {
+        const float mf = (float)largest;
+        odd = !(mf >= kTiny && mf <= kHuge);
+        zero = !(mf > 0.0f && mf < kInf);
+        if (odd) {
+            scale = mf < kTiny ? kScaleTiny : kScaleHuge;
+            m *= (M)scale;
+        }
+        inv = zero ? 0.0f : 127.0f * f2s_rcp_approx((float)m);
+    }
+};
+
+// Two fp32 values in a register pair, and their fused multiply-add.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// 8 values of a thread to 8 bits, in the low bytes of q; at(j): value j in m's
+// type.
+template <typename M, typename F>
+__device__ __forceinline__ void round8(float (&v)[8], const Rounding<M>& r, uint32_t (&q)[8], F at) {
+    if (r.odd) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) q[i] = round8(v[i], inv, off);
-        if (off > kBorder) {
+        for (int j = 0; j < 8; ++j) v[j] *= r.scale;
+    }
+    float off = 0.0f;
+    const uint64_t inv = pair(r.inv, r.inv), magic = pair(kMagic, kMagic), minus = pair(-1.0f, -1.0f);
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                float o = 0.0f;
-                round8(v[i], inv, o);
-                if (o > kBorder) q[i] = round8_exact(at(i), m);
+    for (int j = 0; j < 8; j += 2) {
+        const uint64_t two = pair(v[j], v[j + 1]);
+        const uint64_t shifted = fma2(two, inv, magic);
+        float s0, s1, d0, d1;
+        unpair(shifted, s0, s1);
+        unpair(fma2(two, inv, fma2(shifted, minus, magic)), d0, d1);  // t minus its whole number
+        asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(off) : "f"(off), "f"(d0), "f"(d1));
+        q[j] = __float_as_uint(s0);
+        q[j + 1] = __float_as_uint(s1);
+    }
+    if (off > kBorder) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float whole = __fsub_rn(__uint_as_float(q[j]), kMagic);
+            const float d = __fmaf_rn(v[j], r.inv, -whole);
+            if (fabsf(d) > kBorder) {
+                // the half between `below` and the next whole number
+                const float below = d > 0.0f ? whole : whole - 1.0f;
+                const float side = half_side(at(j), r.m, 2.0f * below + 1.0f);
+                const int k = (int)below;
+                q[j] = (uint32_t)(side > 0.0f || (side == 0.0f && (k & 1)) ? k + 1 : k);
             }
         }
-    } else {
-        const bool tiny = m > 0.0 && m < 1.0;
+    }
+    if (r.zero) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) q[i] = tiny ? round8_exact(at(i), m) : 0u;
+        for (int j = 0; j < 8; ++j) q[j] = 0u;
+    }
+}
+
+// Chunk i of a thread's channels, v, to 8 bits in `row` (of a pitch that keeps
+// vectors aligned where kWide). at(j): value j of the chunk in m's type, scaled.
+template <typename S, bool kWide, typename M, typename F>
+__device__ __forceinline__ void store8_chunk(int8_t* row, int C, int t, int i, float (&v)[8], const Rounding<M>& r,
+                                             F at) {
+    uint32_t q[8];
+    round8(v, r, q, at);
+    const int c = S::channel(i, t);
+    if constexpr (kWide && S::V == 8) {
+        if (c < C)
+            *reinterpret_cast<uint2*>(row + c) =
+                make_uint2(pack_bytes(q[0], q[1], q[2], q[3]), pack_bytes(q[4], q[5], q[6], q[7]));
+    } else if constexpr (kWide) {
+        const int c4 = S::channel(i + 4, t);
+        if (c < C) *reinterpret_cast<uint32_t*>(row + c) = pack_bytes(q[0], q[1], q[2], q[3]);
+        if (c4 < C) *reinterpret_cast<uint32_t*>(row + c4) = pack_bytes(q[4], q[5], q[6], q[7]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (S::channel(i + j, t) < C) row[S::channel(i + j, t)] = (int8_t)(q[j] & 0xffu);
     }
 }
 
@@ -252,63 +387,87 @@ __device__ __forceinline__ void widen8(uint32_t w, float* v) {
 }
 
 // ---- dispatch --------------------------------------------------------------
-// (TPR, E) for a row of C channels: the fewest threads whose 32 registers
-// each hold it, and then the fewest registers. With few rows (fewer threads
-// in all than the SMs hold at one 512-thread block each) more threads per row
-// with 8 registers each shorten the one row's latency instead.
+// What a kernel's registers hold per channel decides how many channels (of
+// `size` bytes) a thread of a TPR-thread row takes at most.
+enum Kind {
+    kForward,  // one or two packed rows
+    kGrad      // s, dy, ds, w and dw; with TPR > 32 the next row's too
+};
+constexpr int most_channels(Kind kind, int size, int tpr) {
+    return kind == kForward ? (size == 2 ? 32 : 16)
+                            : tpr <= 32 ? (size == 2 ? 24 : 16) : (size == 2 ? 16 : 8);
+}
+constexpr int kThreadsForward[] = {8, 32, 128, 512, 1024}, kThreadsGrad[] = {8, 32, 256, 512, 1024};
+
+// (TPR, E) for a row of C channels: the fewest threads that hold it, since each
+// thread's share of the reduction and of the row's constants costs as much as
+// ten channels, and then the fewest registers. Rows past 512 x most_channels
+// take up to 32 channels of 512 or 1,024 threads, and spill a little. With few
+// rows (fewer threads in all than the SMs hold at one 512-thread block each)
+// more threads per row with 8 channels each shorten the one row's latency.
 struct Shape {
     int tpr, e;
 };
 
-inline Shape pick_shape(int64_t nrows, int C, bool wide) {
-    static const int kThreads[] = {8, 32, 128, 512, 1024};
+inline Shape pick_shape(Kind kind, int size, int64_t nrows, int C, bool wide) {
+    const int* threads = kind == kForward ? kThreadsForward : kThreadsGrad;
     int i = 0;
-    while (i < 4 && kThreads[i] * 32 < C) ++i;
-    while (i < 3 && C > kThreads[i] * 8 && nrows * kThreads[i] < (int64_t)sm_count() * 512) ++i;
-    const int e = ceil_div(ceil_div(C, kThreads[i]), 8) * 8;
+    while (i < 3 && threads[i] * most_channels(kind, size, threads[i]) < C) ++i;
+    while (i < 3 && C > threads[i] * 8 && nrows * threads[i] < (int64_t)sm_count() * 512) ++i;
+    if (threads[i] * 32 < C) i = 4;
+    const int e = ceil_div(ceil_div(C, threads[i]), 8) * 8;
     // single values: 8, 16 or 32; 1,024 threads: 32
-    return {kThreads[i], i == 4 || (!wide && e > 16) ? 32 : e};
+    return {threads[i], i == 4 || (!wide && e > 16) ? 32 : e};
+}
+
+// Blocks of `threads` per SM that E channels held in `size` bytes each leave
+// registers for: the second launch bound.
+constexpr int resident(int threads, int E, int size) {
+    return ((E * size <= 32 ? 1536 : 1024) / threads) > 0 ? (E * size <= 32 ? 1536 : 1024) / threads : 1;
 }
 
 // Rows per block and threads per block of a shape.
-inline int block_threads(int tpr) { return tpr <= 32 ? 256 : tpr; }
-inline int block_rows(int tpr) { return tpr <= 32 ? 256 / tpr : 1; }
+constexpr int block_threads(int tpr) { return tpr <= 32 ? 256 : tpr; }
+constexpr int block_rows(int tpr) { return tpr <= 32 ? 256 / tpr : 1; }
+
+template <int kValue>
+using Const = std::integral_constant<int, kValue>;
+
+template <Kind kKind, int kSize, int kTpr, typename F>
+void dispatch_channels(const Shape& s, bool wide, F f) {
+    constexpr int most = kTpr >= 512 ? 32 : most_channels(kKind, kSize, kTpr);
+    if constexpr (kTpr == 1024) {
+        wide ? f(Const<32>(), Const<kTpr>(), std::true_type()) : f(Const<32>(), Const<kTpr>(), std::false_type());
+        return;
+    }
+    if (s.e == 8) wide ? f(Const<8>(), Const<kTpr>(), std::true_type()) : f(Const<8>(), Const<kTpr>(), std::false_type());
+    if constexpr (most >= 16)
+        if (s.e == 16)
+            wide ? f(Const<16>(), Const<kTpr>(), std::true_type()) : f(Const<16>(), Const<kTpr>(), std::false_type());
+    if constexpr (most >= 24)
+        if (s.e == 24 && wide) f(Const<24>(), Const<kTpr>(), std::true_type());
+    if constexpr (most >= 24)  // single values of 24 channels take the kernel of 32
+        if (s.e == 32 && (most >= 32 || !wide)) {
+            if constexpr (most >= 32)
+                if (wide) f(Const<32>(), Const<kTpr>(), std::true_type());
+            if (!wide) f(Const<32>(), Const<kTpr>(), std::false_type());
+        }
+}
+
+// f(E, TPR, wide) for the shape, as integral constants.
+template <Kind kKind, int kSize, typename F>
+void dispatch(const Shape& s, bool wide, F f) {
+    constexpr int kMiddle = kKind == kForward ? 128 : 256;
+    switch (s.tpr) {
+        case 8: dispatch_channels<kKind, kSize, 8>(s, wide, f); break;
+        case 32: dispatch_channels<kKind, kSize, 32>(s, wide, f); break;
+        case kMiddle: dispatch_channels<kKind, kSize, kMiddle>(s, wide, f); break;
+        case 512: dispatch_channels<kKind, kSize, 512>(s, wide, f); break;
+        default: dispatch_channels<kKind, kSize, 1024>(s, wide, f); break;
+    }
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-// F2S_ROW_DISPATCH(shape, wide, T, LAUNCH): LAUNCH(T, E, TPR, kWide) for the
-// shape's constants.
-#define F2S_ROW_E_WIDE(s, T, TPR, LAUNCH)          \
-    switch ((s).e) {                               \
-        case 8: LAUNCH(T, 8, TPR, true); break;    \
-        case 16: LAUNCH(T, 16, TPR, true); break;  \
-        case 24: LAUNCH(T, 24, TPR, true); break;  \
-        default: LAUNCH(T, 32, TPR, true); break;  \
-    }
-#define F2S_ROW_E_SINGLE(s, T, TPR, LAUNCH)         \
-    switch ((s).e) {                                \
-        case 8: LAUNCH(T, 8, TPR, false); break;    \
-        case 16: LAUNCH(T, 16, TPR, false); break;  \
-        default: LAUNCH(T, 32, TPR, false); break;  \
-    }
-#define F2S_ROW_DISPATCH(s, wide, T, LAUNCH)                            \
-    if (wide) {                                                         \
-        switch ((s).tpr) {                                              \
-            case 8: F2S_ROW_E_WIDE(s, T, 8, LAUNCH); break;             \
-            case 32: F2S_ROW_E_WIDE(s, T, 32, LAUNCH); break;           \
-            case 128: F2S_ROW_E_WIDE(s, T, 128, LAUNCH); break;         \
-            case 512: F2S_ROW_E_WIDE(s, T, 512, LAUNCH); break;         \
-            default: LAUNCH(T, 32, 1024, true); break;                  \
-        }                                                               \
-    } else {                                                            \
-        switch ((s).tpr) {                                              \
-            case 8: F2S_ROW_E_SINGLE(s, T, 8, LAUNCH); break;           \
-            case 32: F2S_ROW_E_SINGLE(s, T, 32, LAUNCH); break;         \
-            case 128: F2S_ROW_E_SINGLE(s, T, 128, LAUNCH); break;       \
-            case 512: F2S_ROW_E_SINGLE(s, T, 512, LAUNCH); break;       \
-            default: LAUNCH(T, 32, 1024, false); break;                 \
-        }                                                               \
-    }
 
 // The three element types of these operators (f2s_dtype).
 #define F2S_DTYPE_SWITCH(dtype, ...)                                     \

@@ -10,31 +10,35 @@ namespace {
 using namespace rows;
 
 template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR)
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, sizeof(T)))
 quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t nrows, int width, int8_t* __restrict__ q8,
                      int64_t ldq, float* __restrict__ scale) {
     using S = Slice<T, E, TPR, kWide>;
-    __shared__ uint32_t shared_m[32];
-    __shared__ float shared_a[32];
+    __shared__ float shared_m[32];
     const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
     const int64_t row = TPR <= 32 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
     const bool live = row < nrows;
     const int64_t at = live ? row : 0;
     const int C = live ? width : 0;
-    float v[E];
-    S::load(x + at * ldx, C, t, v);
-    uint32_t m = 0;
-    float unused = 0.0f;
+    const T* from = x + at * ldx;
+    Held<T, E, kWide> held;
+    load_held<S>(from, C, t, held);
+    float m = 0.0f, none = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) m = max(m, abs_bits(v[i]));
-    row_sum_max<TPR>(unused, m, shared_m, shared_a);
-    const float largest = __uint_as_float(m);
-    const bool finite = m < kInfBits;
-    uint32_t q[E];
-    round8_row(v, 127.0f / largest, finite ? (double)largest : 0.0, finite && largest >= kTiny, q,
-               [&](int i) { return (double)v[i]; });
-    S::store8(q8 + at * ldq, C, t, q);
-    if (live && t == 0) scale[row] = finite ? largest / 127.0f : __int_as_float(0x7fc00000);
+    for (int i = 0; i < E; i += 8) {
+        float v[8];
+        held.get(i, v);
+        m = max_abs(v, m);
+    }
+    row_sum_max<TPR, false, true>(none, m, shared_m, shared_m);
+    const Rounding<float> rounding(m);
+#pragma unroll
+    for (int i = 0; i < E; i += 8) {
+        float v[8];
+        held.get(i, v);
+        store8_chunk<S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
+    }
+    if (live && t == 0) scale[row] = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
 }
 
 // y = scale q. kWide: 16 channels per thread (one 16-byte load); else one.
@@ -70,16 +74,14 @@ int quantize_launch(const void* x, int64_t ldx, int64_t nrows, int C, int8_t* q,
     constexpr int vec = kVec<T>;
     const bool wide = C % vec == 0 && aligned16(x) && aligned16(q) &&
                       ((ldx % vec == 0 && ldq % vec == 0) || nrows == 1);
-    const Shape s = pick_shape(nrows, C, wide);
+    const Shape s = pick_shape(kForward, sizeof(T), nrows, C, wide);
     const int64_t blocks = ceil_div64(nrows, block_rows(s.tpr));
     F2S_LIMIT(blocks <= INT32_MAX, "quantize_rows: %lld rows", (long long)nrows);
     TraceScope trace(kTagRows8, st);
-    const T* from = static_cast<const T*>(x);
-#define F2S_LAUNCH(T, E, TPR, W)                                                                   \
-    quantize_rows_kernel<T, E, TPR, W><<<(unsigned)blocks, block_threads(TPR), 0, st>>>(from, ldx, nrows, C, q, ldq, \
-                                                                                        scale)
-    F2S_ROW_DISPATCH(s, wide, T, F2S_LAUNCH);
-#undef F2S_LAUNCH
+    dispatch<kForward, sizeof(T)>(s, wide, [&](auto e, auto tpr, auto w) {
+        quantize_rows_kernel<T, e.value, tpr.value, w.value><<<(unsigned)blocks, block_threads(tpr.value), 0, st>>>(
+            static_cast<const T*>(x), ldx, nrows, C, q, ldq, scale);
+    });
     return check_launch("quantize_rows_kernel");
 }
 

@@ -19,9 +19,9 @@ namespace {
 using namespace rows;
 
 constexpr int kGroup = F2S_SWIGLU_GROUP;
-constexpr int kLanes = 16;                // threads of one group
-constexpr int kEach = kGroup / kLanes;    // channels per thread: 8
-static_assert(kEach == 8, "one 8-byte store of checkpoints per thread");
+constexpr int kLanes = 8;               // threads of one group
+constexpr int kEach = kGroup / kLanes;  // channels per thread: 16
+static_assert(kEach == 16, "one 16-byte store of checkpoints per thread");
 
 // Approximate reciprocal and exponential, 2^-22 relative each: below the
 // rounding of 16-bit results, and 4e-7 relative of fp32 ones.
@@ -29,27 +29,36 @@ __device__ __forceinline__ float sigmoid(float g) {
     return f2s_rcp_approx(1.0f + f2s_ex2_approx(-1.44269504088896341f * g));
 }
 
-// How a thread's 8 channels of a group lie: consecutive where H is a multiple
-// of 8 (with 16-byte accesses where the pointers allow it), else 16 apart, so
-// that a warp's single accesses are adjacent. H alone decides the order, which
-// is also the order of the checkpoint's bytes, in the forward and the backward.
+// v g sigma(g), in one order of products wherever it is computed.
+__device__ __forceinline__ float gated(float g, float v) { return __fmul_rn(__fmul_rn(g, sigmoid(g)), v); }
+
+// How a thread's 16 channels of a group lie: two runs of 8, 64 apart, where H is
+// a multiple of 8 (with 16-byte accesses where the pointers allow it), else
+// single ones, 8 apart, so that a warp's accesses are adjacent. H alone decides
+// the order, which is also the order of the checkpoint's bytes, in the forward
+// and the backward.
 enum Form { kWideRun, kRun, kApart };
+
+template <Form kForm>
+__device__ __forceinline__ int channel_of(int j, int lane) {
+    return kForm == kApart ? j * kLanes + lane : (j / 8) * 64 + lane * 8 + j % 8;
+}
 
 // Channels of a group that begins at `row`; those past `left` (a multiple of 8
 // unless kApart) are outside the row.
 template <typename T, Form kForm>
 __device__ __forceinline__ void load_group(const T* row, int lane, int left, float (&v)[kEach]) {
     if constexpr (kForm == kWideRun) {
-        const bool in = lane * kEach < left;
 #pragma unroll
         for (int j = 0; j < kEach; j += kVec<T>) {
-            const uint4 u = in ? *reinterpret_cast<const uint4*>(row + lane * kEach + j) : make_uint4(0, 0, 0, 0);
+            const int c = channel_of<kForm>(j, lane);
+            const uint4 u = c < left ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
             unpack16<T>(u, &v[j]);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int c = kForm == kRun ? lane * kEach + j : j * kLanes + lane;
+            const int c = channel_of<kForm>(j, lane);
             v[j] = c < left ? to_f32<T>(row[c]) : 0.0f;
         }
     }
@@ -58,44 +67,46 @@ __device__ __forceinline__ void load_group(const T* row, int lane, int left, flo
 template <typename T, Form kForm>
 __device__ __forceinline__ void store_group(T* row, int lane, int left, const float (&v)[kEach]) {
     if constexpr (kForm == kWideRun) {
-        if (lane * kEach >= left) return;
 #pragma unroll
-        for (int j = 0; j < kEach; j += kVec<T>)
-            *reinterpret_cast<uint4*>(row + lane * kEach + j) = pack16<T>(&v[j]);
+        for (int j = 0; j < kEach; j += kVec<T>) {
+            const int c = channel_of<kForm>(j, lane);
+            if (c < left) *reinterpret_cast<uint4*>(row + c) = pack16<T>(&v[j]);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int c = kForm == kRun ? lane * kEach + j : j * kLanes + lane;
+            const int c = channel_of<kForm>(j, lane);
             if (c < left) row[c] = from_f32<T>(v[j]);
         }
     }
 }
 
-// One group's checkpoint: thread `lane` keeps its 8 channels, in its own
-// order, as 8 consecutive bytes.
+// One group's checkpoint: thread `lane` keeps its 16 channels, in its own
+// order, as 16 consecutive bytes.
 __device__ __forceinline__ void keep_group(const float (&v)[kEach], int lane, int8_t* q8, float* scale) {
-    uint32_t m = 0;
+    float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) m = max(m, abs_bits(v[j]));
+    for (int j = 0; j < kEach; j += 2) m = max_abs(m, v[j], v[j + 1]);
+    m = lanes_max<kLanes>(m);
+    const Rounding<float> rounding(m);
+    uint32_t w[kEach / 4];
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float largest = __uint_as_float(m);
-    const bool finite = m < kInfBits;
-    uint32_t q[kEach];
-    round8_row(v, 127.0f / largest, finite ? (double)largest : 0.0, finite && largest >= kTiny, q,
-               [&](int i) { return (double)v[i]; });
-    uint32_t w[2];
+    for (int i = 0; i < kEach; i += 8) {
+        float held[8];
+        uint32_t q[8];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-        w[j] = __byte_perm(__byte_perm(q[4 * j], q[4 * j + 1], 0x0040),
-                           __byte_perm(q[4 * j + 2], q[4 * j + 3], 0x0040), 0x5410);
+        for (int j = 0; j < 8; ++j) held[j] = v[i + j];
+        round8(held, rounding, q, [&](int j) { return held[j]; });
+        w[i / 4] = pack_bytes(q[0], q[1], q[2], q[3]);
+        w[i / 4 + 1] = pack_bytes(q[4], q[5], q[6], q[7]);
+    }
     if (q8) {
-        *reinterpret_cast<uint2*>(q8 + lane * kEach) = make_uint2(w[0], w[1]);
-        if (lane == 0) *scale = finite ? largest / 127.0f : __int_as_float(0x7fc00000);
+        *reinterpret_cast<uint4*>(q8 + lane * kEach) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (lane == 0) *scale = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
     }
 }
 
-// Units of 16 threads, one per (row, group of 128 channels). `kept` of unit u
+// Units of 8 threads, one per (row, group of 128 channels). `kept` of unit u
 // is at byte 256 u (gate, then value), its scales at 2 u.
 template <typename T, Form kForm, bool kKeep>
 __global__ void __launch_bounds__(256)
@@ -113,7 +124,7 @@ swiglu_kernel(const T* __restrict__ projected, int64_t ld, int H, int groups, in
     load_group<T, kForm>(from, lane, left, g);
     load_group<T, kForm>(from + H, lane, left, v);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) h[j] = g[j] * sigmoid(g[j]) * v[j];
+    for (int j = 0; j < kEach; ++j) h[j] = gated(g[j], v[j]);
     store_group<T, kForm>(y + row * (int64_t)H + first, lane, left, h);
     if constexpr (kKeep) {
         // the shuffles need every lane of the warp, live or not
@@ -138,13 +149,17 @@ swiglu_grad_kernel(const T* __restrict__ projected, int64_t ld, const int8_t* __
     load_group<T, kForm>(dy + row * lddy + first, lane, left, d);
     if constexpr (kKept) {
         const int8_t* from = kept + u * (2 * kGroup) + lane * kEach;
-        const uint2 qg = *reinterpret_cast<const uint2*>(from);
-        const uint2 qv = *reinterpret_cast<const uint2*>(from + kGroup);
+        const uint4 qg = *reinterpret_cast<const uint4*>(from);
+        const uint4 qv = *reinterpret_cast<const uint4*>(from + kGroup);
         const float2 s = *reinterpret_cast<const float2*>(scales + 2 * u);
         widen8(qg.x, g);
         widen8(qg.y, g + 4);
+        widen8(qg.z, g + 8);
+        widen8(qg.w, g + 12);
         widen8(qv.x, v);
         widen8(qv.y, v + 4);
+        widen8(qv.z, v + 8);
+        widen8(qv.w, v + 12);
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
             g[j] *= s.x;
@@ -169,35 +184,44 @@ swiglu_grad_kernel(const T* __restrict__ projected, int64_t ld, const int8_t* __
 
 // h as 8-bit rows.
 template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR)
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, 2 * sizeof(T)))
 swiglu_int8_kernel(const T* __restrict__ projected, int64_t ld, int64_t nrows, int H, int8_t* __restrict__ q8,
                    int64_t ldq, float* __restrict__ scale) {
     using S = Slice<T, E, TPR, kWide>;
-    __shared__ uint32_t shared_m[32];
-    __shared__ float shared_a[32];
+    __shared__ float shared_m[32];
     const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
     const int64_t row = TPR <= 32 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
     const bool live = row < nrows;
     const int64_t at = live ? row : 0;
     const int C = live ? H : 0;
-    float h[E], v[E];
-    S::load(projected + at * ld, C, t, h);
-    S::load(projected + at * ld + H, C, t, v);
-    uint32_t m = 0;
-    float unused = 0.0f;
+    const T* from = projected + at * ld;
+    Held<T, E, kWide> gate, value;
+    load_held<S>(from, C, t, gate);
+    load_held<S>(from + H, C, t, value);
+    float h[E];
+    float m = 0.0f, none = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        h[i] = h[i] * sigmoid(h[i]) * v[i];
-        m = max(m, abs_bits(h[i]));
+    for (int i = 0; i < E; i += 8) {
+        float g[8], v[8];
+        gate.get(i, g);
+        value.get(i, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            h[i + j] = gated(g[j], v[j]);
+            v[j] = h[i + j];
+        }
+        m = max_abs(v, m);
     }
-    row_sum_max<TPR>(unused, m, shared_m, shared_a);
-    const float largest = __uint_as_float(m);
-    const bool finite = m < kInfBits;
-    uint32_t q[E];
-    round8_row(h, 127.0f / largest, finite ? (double)largest : 0.0, finite && largest >= kTiny, q,
-               [&](int i) { return (double)h[i]; });
-    S::store8(q8 + at * ldq, C, t, q);
-    if (live && t == 0) scale[row] = finite ? largest / 127.0f : __int_as_float(0x7fc00000);
+    row_sum_max<TPR, false, true>(none, m, shared_m, shared_m);
+    const Rounding<float> rounding(m);
+#pragma unroll
+    for (int i = 0; i < E; i += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = h[i + j];
+        store8_chunk<S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
+    }
+    if (live && t == 0) scale[row] = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
 }
 
 int check_swiglu(const char* what, int dtype, int64_t nrows, int H) {
@@ -227,14 +251,14 @@ int swiglu_launch(const void* projected, int64_t ld, int64_t nrows, int H, void*
                   cudaStream_t st) {
     Units u;
     F2S_TRY(units_of("swiglu", nrows, H, u));
-    const bool wide = H % kEach == 0 && aligned16(projected) && aligned16(y) && (ld % kVec<T> == 0 || nrows == 1);
+    const bool wide = H % 8 == 0 && aligned16(projected) && aligned16(y) && (ld % kVec<T> == 0 || nrows == 1);
     TraceScope trace(kTagSwiGlu, st);
     auto go = [&](auto kernel) {
         kernel<<<u.blocks, 256, 0, st>>>(static_cast<const T*>(projected), ld, H, u.groups, u.units,
                                          static_cast<T*>(y), kept, scales);
     };
     if (wide) kept ? go(swiglu_kernel<T, kWideRun, true>) : go(swiglu_kernel<T, kWideRun, false>);
-    else if (H % kEach == 0) kept ? go(swiglu_kernel<T, kRun, true>) : go(swiglu_kernel<T, kRun, false>);
+    else if (H % 8 == 0) kept ? go(swiglu_kernel<T, kRun, true>) : go(swiglu_kernel<T, kRun, false>);
     else kept ? go(swiglu_kernel<T, kApart, true>) : go(swiglu_kernel<T, kApart, false>);
     return check_launch("swiglu_kernel");
 }
@@ -244,7 +268,7 @@ int swiglu_grad_launch(const void* projected, int64_t ld, const int8_t* kept, co
                        int64_t lddy, int64_t nrows, int H, void* dprojected, cudaStream_t st) {
     Units u;
     F2S_TRY(units_of("swiglu_backward", nrows, H, u));
-    const bool wide = H % kEach == 0 && aligned16(dy) && aligned16(dprojected) && (lddy % kVec<T> == 0 || nrows == 1) &&
+    const bool wide = H % 8 == 0 && aligned16(dy) && aligned16(dprojected) && (lddy % kVec<T> == 0 || nrows == 1) &&
                       (kept || (aligned16(projected) && (ld % kVec<T> == 0 || nrows == 1)));
     TraceScope trace(kTagSwiGlu, st);
     auto go = [&](auto kernel) {
@@ -252,7 +276,7 @@ int swiglu_grad_launch(const void* projected, int64_t ld, const int8_t* kept, co
                                          lddy, H, u.groups, u.units, static_cast<T*>(dprojected));
     };
     if (wide) kept ? go(swiglu_grad_kernel<T, kWideRun, true>) : go(swiglu_grad_kernel<T, kWideRun, false>);
-    else if (H % kEach == 0) kept ? go(swiglu_grad_kernel<T, kRun, true>) : go(swiglu_grad_kernel<T, kRun, false>);
+    else if (H % 8 == 0) kept ? go(swiglu_grad_kernel<T, kRun, true>) : go(swiglu_grad_kernel<T, kRun, false>);
     else kept ? go(swiglu_grad_kernel<T, kApart, true>) : go(swiglu_grad_kernel<T, kApart, false>);
     return check_launch("swiglu_grad_kernel");
 }
@@ -263,15 +287,14 @@ int swiglu_int8_launch(const void* projected, int64_t ld, int64_t nrows, int H, 
     constexpr int vec = kVec<T>;
     const bool wide = H % vec == 0 && aligned16(projected) && aligned16(q) &&
                       ((ld % vec == 0 && ldq % vec == 0) || nrows == 1);
-    const Shape s = pick_shape(nrows, H, wide);
+    const Shape s = pick_shape(kForward, 4, nrows, H, wide);  // h is held in fp32
     const int64_t blocks = ceil_div64(nrows, block_rows(s.tpr));
     F2S_LIMIT(blocks <= INT32_MAX, "swiglu_int8: %lld rows", (long long)nrows);
     TraceScope trace(kTagSwiGlu, st);
-    const T* from = static_cast<const T*>(projected);
-#define F2S_LAUNCH(T, E, TPR, W) \
-    swiglu_int8_kernel<T, E, TPR, W><<<(unsigned)blocks, block_threads(TPR), 0, st>>>(from, ld, nrows, H, q, ldq, scale)
-    F2S_ROW_DISPATCH(s, wide, T, F2S_LAUNCH);
-#undef F2S_LAUNCH
+    dispatch<kForward, 4>(s, wide, [&](auto e, auto tpr, auto w) {
+        swiglu_int8_kernel<T, e.value, tpr.value, w.value><<<(unsigned)blocks, block_threads(tpr.value), 0, st>>>(
+            static_cast<const T*>(projected), ld, nrows, H, q, ldq, scale);
+    });
     return check_launch("swiglu_int8_kernel");
 }
 
@@ -284,8 +307,8 @@ extern "C" int f2s_swiglu(const void* projected, int64_t ld, int dtype, int64_t 
     if (rows == 0) return F2S_OK;
     F2S_REQUIRE(projected && y && (!checkpoint) == (!checkpoint_scale), "swiglu: null pointer");
     F2S_REQUIRE(ld >= 2 * (int64_t)H, "swiglu: row pitch below 2 H = %lld", 2 * (long long)H);
-    F2S_REQUIRE((reinterpret_cast<uintptr_t>(checkpoint) & 7) == 0 && (reinterpret_cast<uintptr_t>(checkpoint_scale) & 7) == 0,
-                "swiglu: checkpoints start on 8 bytes");
+    F2S_REQUIRE((reinterpret_cast<uintptr_t>(checkpoint) & 15) == 0 && (reinterpret_cast<uintptr_t>(checkpoint_scale) & 7) == 0,
+                "swiglu: checkpoints start on 16 bytes");
     int status = F2S_OK;
     F2S_DTYPE_SWITCH(dtype, status = f2s::swiglu_launch<T>(projected, ld, rows, H, y, checkpoint, checkpoint_scale,
                                                            f2s::as_stream(stream)));
@@ -300,8 +323,8 @@ extern "C" int f2s_swiglu_backward(const void* projected, int64_t ld, const int8
     F2S_REQUIRE(dy && dprojected && (projected || checkpoint) && (!checkpoint) == (!checkpoint_scale),
                 "swiglu_backward: null pointer");
     F2S_REQUIRE(lddy >= H && (checkpoint || ld >= 2 * (int64_t)H), "swiglu_backward: row pitch below the row");
-    F2S_REQUIRE((reinterpret_cast<uintptr_t>(checkpoint) & 7) == 0 && (reinterpret_cast<uintptr_t>(checkpoint_scale) & 7) == 0,
-                "swiglu_backward: checkpoints start on 8 bytes");
+    F2S_REQUIRE((reinterpret_cast<uintptr_t>(checkpoint) & 15) == 0 && (reinterpret_cast<uintptr_t>(checkpoint_scale) & 7) == 0,
+                "swiglu_backward: checkpoints start on 16 bytes");
     int status = F2S_OK;
     F2S_DTYPE_SWITCH(dtype, status = f2s::swiglu_grad_launch<T>(projected, ld, checkpoint, checkpoint_scale, dy, lddy,
                                                                 rows, H, dprojected, f2s::as_stream(stream)));
