@@ -397,7 +397,7 @@ constexpr int most_channels(Kind kind, int size, int tpr) {
     return kind == kForward ? (size == 2 ? 32 : 16)
                             : tpr <= 32 ? (size == 2 ? 24 : 16) : (size == 2 ? 16 : 8);
 }
-constexpr int kThreadsForward[] = {8, 32, 128, 512, 1024}, kThreadsGrad[] = {8, 32, 256, 512, 1024};
+constexpr int kThreads[] = {8, 32, 128, 256, 512, 1024};
 
 // (TPR, E) for a row of C channels: the fewest threads that hold it, since each
 // thread's share of the reduction and of the row's constants costs as much as
@@ -410,14 +410,13 @@ struct Shape {
 };
 
 inline Shape pick_shape(Kind kind, int size, int64_t nrows, int C, bool wide) {
-    const int* threads = kind == kForward ? kThreadsForward : kThreadsGrad;
     int i = 0;
-    while (i < 3 && threads[i] * most_channels(kind, size, threads[i]) < C) ++i;
-    while (i < 3 && C > threads[i] * 8 && nrows * threads[i] < (int64_t)sm_count() * 512) ++i;
-    if (threads[i] * 32 < C) i = 4;
-    const int e = ceil_div(ceil_div(C, threads[i]), 8) * 8;
+    while (i < 4 && kThreads[i] * most_channels(kind, size, kThreads[i]) < C) ++i;
+    while (i < 4 && C > kThreads[i] * 8 && nrows * kThreads[i] < (int64_t)sm_count() * 512) ++i;
+    if (kThreads[i] * 32 < C) i = 5;
+    const int e = ceil_div(ceil_div(C, kThreads[i]), 8) * 8;
     // single values: 8, 16 or 32; 1,024 threads: 32
-    return {threads[i], i == 4 || (!wide && e > 16) ? 32 : e};
+    return {kThreads[i], i == 5 || (!wide && e > 16) ? 32 : e};
 }
 
 // Blocks of `threads` per SM that E channels held in `size` bytes each leave
@@ -435,7 +434,7 @@ using Const = std::integral_constant<int, kValue>;
 
 template <Kind kKind, int kSize, int kTpr, typename F>
 void dispatch_channels(const Shape& s, bool wide, F f) {
-    constexpr int most = kTpr >= 512 ? 32 : most_channels(kKind, kSize, kTpr);
+    constexpr int most = kTpr == 512 ? 32 : most_channels(kKind, kSize, kTpr);
     if constexpr (kTpr == 1024) {
         wide ? f(Const<32>(), Const<kTpr>(), std::true_type()) : f(Const<32>(), Const<kTpr>(), std::false_type());
         return;
@@ -457,11 +456,11 @@ void dispatch_channels(const Shape& s, bool wide, F f) {
 // f(E, TPR, wide) for the shape, as integral constants.
 template <Kind kKind, int kSize, typename F>
 void dispatch(const Shape& s, bool wide, F f) {
-    constexpr int kMiddle = kKind == kForward ? 128 : 256;
     switch (s.tpr) {
         case 8: dispatch_channels<kKind, kSize, 8>(s, wide, f); break;
         case 32: dispatch_channels<kKind, kSize, 32>(s, wide, f); break;
-        case kMiddle: dispatch_channels<kKind, kSize, kMiddle>(s, wide, f); break;
+        case 128: dispatch_channels<kKind, kSize, 128>(s, wide, f); break;
+        case 256: dispatch_channels<kKind, kSize, 256>(s, wide, f); break;
         case 512: dispatch_channels<kKind, kSize, 512>(s, wide, f); break;
         default: dispatch_channels<kKind, kSize, 1024>(s, wide, f); break;
     }
