@@ -2,8 +2,10 @@
 
 Objects go to _build/ beside this file; the shared library lands inside the
 Python package (flow2surf_b200/libflow2surf_sm100.so) so that it travels with
-the source tree. Only sources newer than their object (or than any header) are
-recompiled.
+the source tree, and so does the PyTorch binding of the 8-bit feed-forward
+operators (flow2surf_b200/_feedforward.so, from csrc/feedforward_torch.cpp with
+the host compiler). Only sources newer than their object (or than any header)
+are recompiled.
 
     python jittor-flow2surf_b200/build.py [--force] [--jobs N]
 """
@@ -15,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -24,6 +27,8 @@ CSRC = HERE / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = HERE / "_build"
 LIBRARY = HERE / "flow2surf_b200" / "libflow2surf_sm100.so"
+BINDING_SOURCE = CSRC / "feedforward_torch.cpp"
+BINDING = HERE / "flow2surf_b200" / "_feedforward.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -65,6 +70,33 @@ def _compile(src: Path, force: bool, extra: list[str]) -> tuple[Path, str]:
     return obj, proc.stderr
 
 
+def _build_binding(force: bool) -> None:
+    """The PyTorch binding, against the torch of this interpreter (a stamp in
+    _build/ names its version)."""
+    import torch
+
+    stamp = BUILD / "feedforward_torch.stamp"
+    wanted = f"{torch.__version__} {sys.version}"
+    inputs = [BINDING_SOURCE, *INCLUDE.glob("*.h")]
+    if (not force and BINDING.exists() and stamp.exists() and stamp.read_text() == wanted
+            and BINDING.stat().st_mtime >= max(i.stat().st_mtime for i in inputs)):
+        return
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{INCLUDE}", "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
+           str(BINDING_SOURCE), "-o", str(BINDING), f"-L{LIBRARY.parent}", f"-l:{LIBRARY.name}",
+           "-Wl,-rpath,$ORIGIN", f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {BINDING_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
+    stamp.write_text(wanted)
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
           extra: list[str] | None = None) -> Path:
     BUILD.mkdir(exist_ok=True)
@@ -84,6 +116,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
+    _build_binding(force)
     return LIBRARY
 
 
