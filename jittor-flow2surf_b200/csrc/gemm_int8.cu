@@ -53,8 +53,9 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t a, uint32_t r) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(r));
     return d;
 }
-__device__ __forceinline__ void store_cluster(uint32_t a, int v) {
-    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+__device__ __forceinline__ void store_cluster(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
 }
 
 template <typename T>
@@ -87,7 +88,7 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int S = g.stages;
-    int* partial = reinterpret_cast<int*>(smem + (size_t)S * kStage);  // [split][BN / split][128]
+    int4* partial = reinterpret_cast<int4*>(smem + (size_t)S * kStage);  // [split][BN / split / 4][128] of 4 tokens
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * kStage + (g.split > 1 ? BN * 512 : 0));
     uint64_t* empty = full + S;
     uint64_t* done = empty + S;
@@ -178,8 +179,8 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         }
         ok = __all_sync(0xffffffffu, tc::mbar_wait_poll(done, 0, g.err));
         tc::tc_fence_after();
-        const int own = BN / split;  // tokens that each CTA of the cluster finishes
-        const int shift = __ffs(own) - 1;
+        // each CTA of the cluster finishes BN / split tokens, in fours
+        const int own = BN / 4 / split, shift = __ffs(own) - 1;
         const uint32_t mine = tc::smem_u32(partial + rank * own * 128 + channel);
 #pragma unroll
         for (int j0 = 0; j0 < BN; j0 += kStep) {
@@ -201,9 +202,9 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < kStep; ++j) {
-                    const uint32_t to = (uint32_t)(j0 + j) >> shift;
-                    store_cluster(map_rank(mine + ((uint32_t)(j0 + j) & (own - 1)) * 512u, to), (int)v[j]);
+                for (int j = 0; j < kStep; j += 4) {
+                    const uint32_t four = (uint32_t)(j0 + j) / 4, to = four >> shift;
+                    store_cluster(map_rank(mine + (four & (own - 1)) * 2048u, to), v[j], v[j + 1], v[j + 2], v[j + 3]);
                 }
             }
         }
@@ -212,13 +213,22 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         cluster_arrive();
         cluster_wait();
         if (warp >= 2 && ok && n < g.cols) {
-            const int own = BN / split;
+            const int own = BN / 4 / split;
             for (int j = 0; j < own; ++j) {
-                const int m = m0 + rank * own + j;
+                const int m = m0 + (rank * own + j) * 4;
                 if (m >= g.rows) break;
-                int acc = 0;
-                for (int r = 0; r < split; ++r) acc += partial[(r * own + j) * 128 + channel];
-                store(m, acc, ws, b);
+                int4 acc = partial[j * 128 + channel];
+                for (int r = 1; r < split; ++r) {
+                    const int4 more = partial[(r * own + j) * 128 + channel];
+                    acc.x += more.x;
+                    acc.y += more.y;
+                    acc.z += more.z;
+                    acc.w += more.w;
+                }
+                store(m, acc.x, ws, b);
+                if (m + 1 < g.rows) store(m + 1, acc.y, ws, b);
+                if (m + 2 < g.rows) store(m + 2, acc.z, ws, b);
+                if (m + 3 < g.rows) store(m + 3, acc.w, ws, b);
             }
         }
     }
@@ -274,6 +284,19 @@ int tiles_launch(const Int8Args& a, int split, cudaStream_t st) {
 
 // ---- pairs -------------------------------------------------------------------
 
+struct PairArgs;
+
+// A pair's output tiles: t, t + pairs, ... of an order in bands of 8 token
+// tiles, channels outer, so that the operands of the tiles that run at one
+// time stay in L2. Advanced by additions: a division costs a warp as much as
+// the arithmetic of ten output columns.
+struct Walk {
+    int t, band, in_band;
+    __device__ __forceinline__ void start(const PairArgs& g, int first);
+    __device__ __forceinline__ void next(const PairArgs& g, int pairs);
+    __device__ __forceinline__ void at(const PairArgs& g, int& m0, int& n0) const;
+};
+
 struct PairArgs {
     const float* xs;
     const float* ws;
@@ -284,13 +307,34 @@ struct PairArgs {
     int bn;          // channels of a tile: 64, 128, 192 or 256
     int k_blocks, stages;
     int m_tiles, n_tiles;
+    int step_bands, step_rest;  // the number of pairs, in bands and tiles
     int boxes;       // y written by TMA
     uint32_t idesc;
     int* err;
 };
 
-constexpr int kPairEpilogue = 256;  // 8 warps
-constexpr int kPairThreads = 64 + kPairEpilogue;
+__device__ __forceinline__ void Walk::start(const PairArgs& g, int first) {
+    t = first;
+    band = first / (8 * g.n_tiles);
+    in_band = first - band * 8 * g.n_tiles;
+}
+__device__ __forceinline__ void Walk::next(const PairArgs& g, int pairs) {
+    t += pairs;
+    band += g.step_bands;
+    in_band += g.step_rest;
+    if (in_band >= 8 * g.n_tiles) {
+        in_band -= 8 * g.n_tiles;
+        ++band;
+    }
+}
+__device__ __forceinline__ void Walk::at(const PairArgs& g, int& m0, int& n0) const {
+    const int high = g.m_tiles - band * 8;  // of the last band, if below 8
+    const int n = high >= 8 ? in_band >> 3 : in_band / high;
+    m0 = (band * 8 + in_band - n * (high >= 8 ? 8 : high)) * 256;
+    n0 = n * g.bn;
+}
+
+constexpr int kPairThreads = 64 + 32 * 8;
 constexpr int kBox = 32 * 128;      // 32 rows of 128 bytes of y
 
 // TMA load by either CTA of a pair, signalling a barrier of the pair's leader.
@@ -319,59 +363,42 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
         : "memory");
 }
 
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrive on a barrier of either CTA of the pair. Only tensor memory is handed
+// over, ordered by the tcgen05 fences around it: a release of cluster scope would
+// wait for this thread's stores of y first, 1 us a tile.
+__device__ __forceinline__ void arrive_pair(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Bounded wait as tc::mbar_wait_poll, for arrivals from the other CTA too.
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
-    for (uint32_t i = 0; i < tc::kSpinLimit; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(tc::smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((i & 63u) == 63u && *reinterpret_cast<volatile int*>(err) != tc::kTcOk) return false;
-    }
-    atomicExch(err, tc::kTcWaitTimeout);
-    return false;
-}
-
+// Eight epilogue warps, two per TMEM lane quarter with every other box of 128
+// bytes of y. (Sixteen, on two accumulators by turns, were slower: 64 us against
+// 58 for 65,536 x 192 -> 1,536, at 96 registers a thread.)
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                          const __grid_constant__ CUtensorMap map_y, const PairArgs g) {
     constexpr int kBoxCols = 128 / (int)sizeof(T);
+    constexpr int kWarps = 8;
+    constexpr int kCols = 128;  // columns of a warp
     extern __shared__ unsigned char raw[];
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int S = g.stages;
     const uint32_t a_bytes = 128 * 128, b_bytes = (uint32_t)g.bn * 64, stage_bytes = a_bytes + b_bytes;
-    unsigned char* boxes = smem + (size_t)S * stage_bytes;                    // 8 warps x kBox
-    float* vectors = reinterpret_cast<float*>(boxes + 8 * kBox);               // 8 warps x [ws 128 | bias 128]
-    uint64_t* full = reinterpret_cast<uint64_t*>(vectors + 8 * 256);          // leader's: both CTAs' bytes
+    unsigned char* boxes = smem + (size_t)S * stage_bytes;  // kWarps x kBox
+    float* vectors = reinterpret_cast<float*>(boxes + kWarps * kBox);  // a warp's [ws kCols | bias kCols]
+    uint64_t* full = reinterpret_cast<uint64_t*>(vectors + kWarps * 2 * kCols);  // leader's: both CTAs' bytes
     uint64_t* empty = full + S;
     uint64_t* tfull = empty + S;   // [2]
-    uint64_t* tempty = tfull + 2;  // [2] leader's: 16 epilogue warps of both CTAs
+    uint64_t* tempty = tfull + 2;  // [2] leader's: eight epilogue warps of both CTAs
     uint64_t* done = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int tiles = g.m_tiles * g.n_tiles, pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
-    // tiles in bands of 8 token tiles, channels outer: the operands of the
-    // tiles that run at one time stay in L2
-    auto tile_at = [&](int t, int& m0, int& n0) {
-        const int per_band = 8 * g.n_tiles, band = t / per_band, r = t - band * per_band;
-        const int high = g.m_tiles - band * 8 < 8 ? g.m_tiles - band * 8 : 8;
-        const int n = r / high;
-        m0 = (band * 8 + r - n * high) * 256;
-        n0 = n * g.bn;
-    };
+    Walk walk;
+    walk.start(g, pair);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -405,11 +432,11 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             int stage = 0;
             uint32_t phase = 0, pending = 0, pending_phase = 0;
             bool ok = true;
-            for (int t = pair; ok && t < tiles; t += pairs) {
+            for (; ok && walk.t < tiles; walk.next(g, pairs)) {
                 int m0, n0;
-                tile_at(t, m0, n0);
+                walk.at(g, m0, n0);
                 for (int kb = 0; kb < g.k_blocks; ++kb) {
-                    if (!wait_cluster(&empty[stage], phase ^ 1u, g.err)) {
+                    if (!tc::mbar_wait_poll(&empty[stage], phase ^ 1u, g.err)) {
                         ok = false;
                         break;
                     }
@@ -444,11 +471,11 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             bool ok = true;
             for (int t = pair; ok && t < tiles; t += pairs, ++iter) {
                 const int buf = iter & 1;
-                if (!wait_cluster(&tempty[buf], ((uint32_t)(iter >> 1) & 1u) ^ 1u, g.err)) break;
+                if (!tc::mbar_wait_poll(&tempty[buf], ((uint32_t)(iter >> 1) & 1u) ^ 1u, g.err)) break;
                 tc::tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)(buf * 256);
                 for (int kb = 0; kb < g.k_blocks; ++kb) {
-                    if (!wait_cluster(&full[stage], phase, g.err)) {
+                    if (!tc::mbar_wait_poll(&full[stage], phase, g.err)) {
                         ok = false;
                         break;
                     }
@@ -470,29 +497,45 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         }
         __syncwarp();
     } else {
-        const int e = warp - 2;        // 0 .. 7
-        const int quarter = warp & 3;  // TMEM lanes of this warp
-        const int half = e >> 2;       // boxes half, half + 2, ...
+        const int e = warp - 2;
+        const int quarter = warp & 3;      // TMEM lanes of this warp
+        const int half = e >> 2;           // boxes half, half + 2, ...
         unsigned char* box = boxes + e * kBox;
-        float* ws = vectors + e * 256;
-        float* bs = ws + 128;
-        int iter = 0;
-        for (int t = pair; t < tiles; t += pairs, ++iter) {
-            int m0, n0;
-            tile_at(t, m0, n0);
-            const int buf = iter & 1;
-            const int row0 = m0 + (int)rank * 128 + quarter * 32, row = row0 + lane;
-            // the scales and biases of this warp's columns (box by box), for
-            // this warp alone: no barrier that another warp could miss
+        float* ws = vectors + e * 2 * kCols;
+        float* bs = ws + kCols;
+        const uint32_t to_leader[2] = {map_rank(tc::smem_u32(&tempty[0]), 0), map_rank(tc::smem_u32(&tempty[1]), 0)};
+        // a tile's token scale and the scales and biases of this warp's columns
+        // (box by box), on their way while the tile before is written; for this
+        // warp alone, so there is no barrier that another warp could miss. Past
+        // the last row or column: the last one's, not written.
+        int m0 = 0, n0 = 0;
+        float xs_next = 0.0f, ws_next[kCols / 32], bs_next[kCols / 32];
+        auto fetch = [&]() {
+            if (walk.t >= tiles) return;
+            walk.at(g, m0, n0);
+            xs_next = __ldg(g.xs + min(m0 + (int)rank * 128 + quarter * 32 + lane, g.rows - 1));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int l = lane + 32 * i, n = n0 + (half + 2 * (l / kBoxCols)) * kBoxCols + l % kBoxCols;
-                ws[l] = n < g.cols ? __ldg(g.ws + n) : 0.0f;
-                bs[l] = n < g.cols ? bias_at<T>(g.bias, n) : 0.0f;
+            for (int i = 0; i < kCols / 32; ++i) {
+                const int l = lane + 32 * i;
+                const int n = min(n0 + (half + 2 * (l / kBoxCols)) * kBoxCols + l % kBoxCols, g.cols - 1);
+                ws_next[i] = __ldg(g.ws + n);
+                bs_next[i] = bias_at<T>(g.bias, n);
+            }
+        };
+        fetch();
+        for (int t = pair, iter = 0; t < tiles; t += pairs, ++iter) {
+            const int buf = iter & 1;
+            const int row0 = m0 + (int)rank * 128 + quarter * 32, col0 = n0;
+            const float xs = xs_next;
+#pragma unroll
+            for (int i = 0; i < kCols / 32; ++i) {
+                ws[lane + 32 * i] = ws_next[i];
+                bs[lane + 32 * i] = bs_next[i];
             }
             __syncwarp();
-            const float xs = row < g.rows ? __ldg(g.xs + row) : 0.0f;
-            const bool ok = wait_cluster(&tfull[buf], (uint32_t)(iter >> 1) & 1u, g.err);
+            walk.next(g, pairs);
+            fetch();
+            const bool ok = tc::mbar_wait_poll(&tfull[buf], (uint32_t)(iter >> 1) & 1u, g.err);
             // a warp that gave up stops with its lanes together
             if (!__all_sync(0xffffffffu, ok)) break;
             tc::tc_fence_after();
@@ -528,9 +571,9 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     // this warp's last read of the accumulator
                     tc::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) arrive_cluster(map_rank(tc::smem_u32(&tempty[buf]), 0));
+                    if (lane == 0) arrive_pair(to_leader[buf]);
                 }
-                if (n0 + c >= g.cols) continue;  // past the last column
+                if (col0 + c >= g.cols) continue;  // past the last column
                 // the previous store has read this box
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
@@ -544,7 +587,7 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     if (lane == 0) {
                         asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                                          reinterpret_cast<uint64_t>(&map_y)),
-                                     "r"(tc::smem_u32(box)), "r"(n0 + c), "r"(row0)
+                                     "r"(tc::smem_u32(box)), "r"(col0 + c), "r"(row0)
                                      : "memory");
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
@@ -553,21 +596,21 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     __syncwarp();
                     const T* held = reinterpret_cast<const T*>(box);
                     for (int r = 0; r < 32 && row0 + r < g.rows; ++r) {
-                        T* to = static_cast<T*>(g.y) + (int64_t)(row0 + r) * g.ldy + n0 + c;
+                        T* to = static_cast<T*>(g.y) + (int64_t)(row0 + r) * g.ldy + col0 + c;
 #pragma unroll
                         for (int k = lane; k < kBoxCols; k += 32) {
                             const int chunk = k * (int)sizeof(T) / 16, in = k % (16 / (int)sizeof(T));
-                            if (n0 + c + k < g.cols)
+                            if (col0 + c + k < g.cols)
                                 to[k] = held[(r * 128 + ((chunk ^ (r & 7)) << 4)) / (int)sizeof(T) + in];
                         }
                     }
                 }
             }
-            // a warp without a box in this tile (bn of one box) frees its share too
+            // a warp without a box in this tile frees its share too
             if (half * kBoxCols >= g.bn) {
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_cluster(map_rank(tc::smem_u32(&tempty[buf]), 0));
+                if (lane == 0) arrive_pair(to_leader[buf]);
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -613,14 +656,16 @@ int pairs_launch(const Int8Args& a, int bn, cudaStream_t st) {
                                          128 / (int)sizeof(T)));
     else my = mx;
     const size_t stage = 128 * 128 + (size_t)bn * 64;
-    const size_t fixed = 1024 + 8 * kBox + 8 * 256 * sizeof(float) + 512;
+    const size_t fixed = 1024 + 8 * (kBox + 2 * 128 * sizeof(float)) + 512;
     int stages = (int)((kSmemLimit - fixed) / stage);
     g.stages = stages > 8 ? 8 : stages;
     const size_t smem = fixed + g.stages * stage;
     auto kernel = linear_int8_pairs_kernel<T>;
     F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int tiles = g.m_tiles * g.n_tiles, pairs = sm_count() / 2;
-    kernel<<<2 * (tiles < pairs ? tiles : pairs), kPairThreads, smem, st>>>(mx, mw, my, g);
+    const int tiles = g.m_tiles * g.n_tiles, most = sm_count() / 2, pairs = tiles < most ? tiles : most;
+    g.step_bands = pairs / (8 * g.n_tiles);
+    g.step_rest = pairs % (8 * g.n_tiles);
+    kernel<<<2 * pairs, kPairThreads, smem, st>>>(mx, mw, my, g);
     return check_launch("linear_int8_pairs_kernel");
 }
 
@@ -633,7 +678,7 @@ int linear_int8_tiles(const Int8Args& a, cudaStream_t st) {
     const int64_t ctas = (int64_t)ceil_div(a.cols, 128) * ceil_div(a.rows, bn);
     const int k_blocks = ceil_div(a.K, kBlockK);
     int split = 1;
-    while (split < 8 && ctas * split < sm_count() && k_blocks >= 4 * split) split *= 2;
+    while (split < 8 && split < bn / 4 && ctas * split < sm_count() && k_blocks >= 4 * split) split *= 2;
     int status = F2S_OK;
     F2S_DTYPE_SWITCH(a.dtype, switch (bn) {
         case 16: status = tiles_launch<T, 16>(a, split, st); break;

@@ -1,6 +1,7 @@
 // Product of 8-bit integer rows with scales for each token and channel:
 //   y[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k] + b[n],
 // the sum exact in 32 bits (K <= 131,071 keeps 2^14 K below 2^31).
+#include <stdlib.h>
 #include "gemm_int8.cuh"
 #include "row_ops.cuh"
 
@@ -10,6 +11,80 @@ namespace {
 using namespace rows;
 
 constexpr int kMaxK = 131071;
+
+// A few tokens: bound by the weights' bytes and by latency. A warp takes two
+// channels (and 1 / kSplit of their K, joined in shared memory), 16 bytes of
+// each per lane and step, four products and sums per dp4a; its loads of several
+// steps are in flight at once.
+constexpr int kFew = 8;        // tokens at most
+constexpr int kFewWarps = 8;   // per block
+
+template <typename T, int R>
+__global__ void __launch_bounds__(32 * kFewWarps) linear_int8_few_kernel(const Int8Args g, int split) {
+    __shared__ int sums[kFewWarps][2 * R];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = warp / split, part = warp - group * split;
+    const int n0 = ((int)blockIdx.x * (kFewWarps / split) + group) * 2;
+    const int chunks = g.K / 16;  // whole 16-byte chunks
+    const int c0 = (int)((int64_t)part * chunks / split), c1 = (int)((int64_t)(part + 1) * chunks / split);
+    int acc[2][R] = {};
+    // a channel past the last one reads the last one and is not written
+    const int8_t* w0 = g.w + (int64_t)(n0 < g.cols ? n0 : g.cols - 1) * g.ldw;
+    const int8_t* w1 = g.w + (int64_t)(n0 + 1 < g.cols ? n0 + 1 : g.cols - 1) * g.ldw;
+#pragma unroll 4
+    for (int c = c0 + lane; c < c1; c += 32) {
+        const int4 a = __ldg(reinterpret_cast<const int4*>(w0) + c), b = __ldg(reinterpret_cast<const int4*>(w1) + c);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (r >= g.rows) break;
+            const int4 x = __ldg(reinterpret_cast<const int4*>(g.x + r * g.ldx) + c);
+            acc[0][r] = __dp4a(a.w, x.w, __dp4a(a.z, x.z, __dp4a(a.y, x.y, __dp4a(a.x, x.x, acc[0][r]))));
+            acc[1][r] = __dp4a(b.w, x.w, __dp4a(b.z, x.z, __dp4a(b.y, x.y, __dp4a(b.x, x.x, acc[1][r]))));
+        }
+    }
+    // the bytes past the last whole chunk, one per lane of the first part
+    const int k = chunks * 16 + lane;
+    if (part == 0 && k < g.K) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (r >= g.rows) break;
+            const int x = g.x[r * g.ldx + k];
+            acc[0][r] += w0[k] * x;
+            acc[1][r] += w1[k] * x;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) {
+        const int sum = __reduce_add_sync(0xffffffffu, acc[i & 1][i >> 1]);
+        if (lane == 0) sums[warp][i] = sum;
+    }
+    if (split > 1) __syncthreads();
+    else __syncwarp();
+    if (part == 0 && lane < 2 * R) {
+        const int n = n0 + (lane & 1), r = lane >> 1;
+        if (n < g.cols && r < g.rows) {
+            int sum = 0;
+            for (int p = 0; p < split; ++p) sum += sums[warp + p][lane];
+            const float b = g.bias ? to_f32<T>(static_cast<const T*>(g.bias)[n]) : 0.0f;
+            static_cast<T*>(g.y)[r * g.ldy + n] = from_f32<T>(fmaf((float)sum * g.xs[r], g.ws[n], b));
+        }
+    }
+}
+
+template <typename T>
+int few_launch(const Int8Args& g, cudaStream_t st) {
+    // K split until every SM has 16 warps, at least two steps each
+    int split = 1;
+    while (split < kFewWarps && (int64_t)ceil_div(g.cols, 2) * split < 16 * sm_count() && g.K >= 2 * 512 * 2 * split)
+        split *= 2;
+    const int blocks = ceil_div(g.cols, 2 * (kFewWarps / split));
+    auto go = [&](auto kernel) { kernel<<<blocks, 32 * kFewWarps, 0, st>>>(g, split); };
+    if (g.rows == 1) go(linear_int8_few_kernel<T, 1>);
+    else if (g.rows == 2) go(linear_int8_few_kernel<T, 2>);
+    else if (g.rows <= 4) go(linear_int8_few_kernel<T, 4>);
+    else go(linear_int8_few_kernel<T, 8>);
+    return check_launch("linear_int8_few_kernel");
+}
 
 // Any pitch and alignment: 64 x 64 outputs per block of 256 threads, 4 x 4
 // each, K in steps of 64 staged in shared memory as words of four, four
@@ -82,7 +157,17 @@ extern "C" int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scal
     f2s::TraceScope trace(f2s::kTagGemmInt8, st);
     using f2s::rows::aligned16;
     if (aligned16(x) && aligned16(w) && (ldx % 16 == 0 || rows == 1) && (ldw % 16 == 0 || cols == 1))
+    {
+        const char* form = getenv("F2S_FORM");
+        if (form && *form == 't') return f2s::linear_int8_tiles(g, st);
+        if (form && *form == 'p') return f2s::linear_int8_pairs(g, st);
+        if ((form && *form == 'f') || (!form && rows <= 4)) {
+            int status = F2S_OK;
+            F2S_DTYPE_SWITCH(dtype, status = f2s::few_launch<T>(g, st));
+            return status;
+        }
         return rows >= 1024 ? f2s::linear_int8_pairs(g, st) : f2s::linear_int8_tiles(g, st);
+    }
     int status = F2S_OK;
     F2S_DTYPE_SWITCH(dtype, status = f2s::any_launch<T>(g, st));
     return status;
