@@ -72,7 +72,7 @@ struct TileArgs {
     void* y;
     int64_t ldy;
     int rows, cols;
-    int k_blocks, stages, split;
+    int k_blocks, stages, split, partial_bytes;
     int* err;
 };
 
@@ -88,8 +88,8 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int S = g.stages;
-    int4* partial = reinterpret_cast<int4*>(smem + (size_t)S * kStage);  // [split][BN / split / 4][128] of 4 tokens
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * kStage + (g.split > 1 ? BN * 512 : 0));
+    int4* partial = reinterpret_cast<int4*>(smem + (size_t)S * kStage);  // [own][split][128] of 4 tokens
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * kStage + g.partial_bytes);
     uint64_t* empty = full + S;
     uint64_t* done = empty + S;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -101,6 +101,14 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     const int kb0 = (int)((int64_t)rank * g.k_blocks / split);
     const int kb1 = (int)((int64_t)(rank + 1) * g.k_blocks / split);
 
+    auto load = [&](int i) {
+        const int s = i % S;
+        unsigned char* st = smem + (size_t)s * kStage;
+        tc::mbar_arrive_expect_tx(&full[s], kStage);
+        tc::tma_load_2d(st, &map_w, &full[s], (kb0 + i) * kBlockK, n0);
+        tc::tma_load_2d(st + kA, &map_x, &full[s], (kb0 + i) * kBlockK, m0);
+    };
+    const int blocks = kb1 - kb0, ahead = min(min(blocks, S), 2);
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             tc::mbar_init(&full[s], 1);
@@ -108,8 +116,9 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         }
         tc::mbar_init(done, 1);
         tc::fence_barrier_init();
-        tc::prefetch_tensormap(&map_w);
-        tc::prefetch_tensormap(&map_x);
+        // the first blocks are on their way while the CTA sets up (an issue takes
+        // 0.1 us and more: all of a ring's would hold the other warps up)
+        for (int i = 0; i < ahead; ++i) load(i);
     }
     if (warp == 1) tc::tmem_alloc(tmem_slot, kCols);
     tc::tc_fence_before();
@@ -121,26 +130,14 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t pending = 0, pending_phase = 0;
-            bool ok = true;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const int i = kb - kb0, s = i % S;
-                const uint32_t phase = (uint32_t)(i / S) & 1u;
-                if (!tc::mbar_wait(&empty[s], phase ^ 1u, g.err)) {
-                    ok = false;
+            for (int i = ahead; i < blocks; ++i) {
+                if (i >= S && !tc::mbar_wait_poll(&empty[i % S], ((uint32_t)(i / S) & 1u) ^ 1u, g.err)) {
+                    // let the copies already issued land before the CTA exits:
+                    // each stage's last one
+                    for (int j = i - S; j < i; ++j) tc::mbar_drain(&full[j % S], (uint32_t)(j / S) & 1u);
                     break;
                 }
-                unsigned char* st = smem + (size_t)s * kStage;
-                tc::mbar_arrive_expect_tx(&full[s], kStage);
-                tc::tma_load_2d(st, &map_w, &full[s], kb * kBlockK, n0);
-                tc::tma_load_2d(st + kA, &map_x, &full[s], kb * kBlockK, m0);
-                pending |= 1u << s;
-                pending_phase = (pending_phase & ~(1u << s)) | (phase << s);
-            }
-            if (!ok) {
-                // let the copies already issued land before the CTA exits
-                for (int s = 0; s < S; ++s)
-                    if (pending & (1u << s)) tc::mbar_drain(&full[s], (pending_phase >> s) & 1u);
+                load(i);
             }
         }
         __syncwarp();
@@ -179,9 +176,9 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         }
         ok = __all_sync(0xffffffffu, tc::mbar_wait_poll(done, 0, g.err));
         tc::tc_fence_after();
-        // each CTA of the cluster finishes BN / split tokens, in fours
-        const int own = BN / 4 / split, shift = __ffs(own) - 1;
-        const uint32_t mine = tc::smem_u32(partial + rank * own * 128 + channel);
+        // four tokens at a time go to the CTAs of the cluster in turn, which
+        // finish them
+        const uint32_t mine = tc::smem_u32(partial + rank * 128 + channel);
 #pragma unroll
         for (int j0 = 0; j0 < BN; j0 += kStep) {
             uint32_t v[kStep];
@@ -203,8 +200,10 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
             } else {
 #pragma unroll
                 for (int j = 0; j < kStep; j += 4) {
-                    const uint32_t four = (uint32_t)(j0 + j) / 4, to = four >> shift;
-                    store_cluster(map_rank(mine + (four & (own - 1)) * 2048u, to), v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    // split is a power of two
+                    const uint32_t four = (uint32_t)(j0 + j) / 4, to = four & (split - 1);
+                    store_cluster(map_rank(mine + (four & ~(uint32_t)(split - 1)) * 2048u, to), v[j], v[j + 1],
+                                  v[j + 2], v[j + 3]);
                 }
             }
         }
@@ -213,13 +212,13 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         cluster_arrive();
         cluster_wait();
         if (warp >= 2 && ok && n < g.cols) {
-            const int own = BN / 4 / split;
-            for (int j = 0; j < own; ++j) {
-                const int m = m0 + (rank * own + j) * 4;
+            for (int four = rank; four < BN / 4; four += split) {
+                const int m = m0 + four * 4;
                 if (m >= g.rows) break;
-                int4 acc = partial[j * 128 + channel];
+                const int4* from = partial + (four - rank) * 128 + channel;
+                int4 acc = from[0];
                 for (int r = 1; r < split; ++r) {
-                    const int4 more = partial[(r * own + j) * 128 + channel];
+                    const int4 more = from[r * 128];
                     acc.x += more.x;
                     acc.y += more.y;
                     acc.z += more.z;
@@ -249,14 +248,16 @@ int tiles_launch(const Int8Args& a, int split, cudaStream_t st) {
     CUtensorMap mw, mx;
     F2S_TRY(operand_map(&mw, a.w, a.ldw, a.cols, a.K, 128));
     F2S_TRY(operand_map(&mx, a.x, a.ldx, a.rows, a.K, BN));
-    TileArgs g{a.xs, a.ws, a.bias, a.y, a.ldy, a.rows, a.cols, ceil_div(a.K, kBlockK), 0, split, tc_error_word()};
+    // fours of tokens per CTA, from every CTA of the cluster
+    const int partial = split > 1 ? ceil_div(BN / 4, split) * split * 128 * 16 : 0;
+    TileArgs g{a.xs, a.ws, a.bias, a.y, a.ldy, a.rows, a.cols, ceil_div(a.K, kBlockK), 0, split, partial, tc_error_word()};
     if (!g.err) return fail(F2S_ERR_CUDA, "linear_int8: device error word unavailable");
     const size_t stage = 128 * 128 + BN * 128;
-    const size_t fixed = 1024 + 512 + (split > 1 ? BN * 512 : 0);
+    const size_t fixed = 1024 + 512 + partial;
     // two CTAs per SM where there are that many
     const int per_cta = ceil_div(g.k_blocks, split);
     const int64_t ctas = (int64_t)ceil_div(a.cols, 128) * split * ceil_div(a.rows, BN);
-    const size_t budget = BN < 128 && ctas > sm_count() ? kSmemLimit / 2 - 1024 : kSmemLimit;
+    const size_t budget = ctas > sm_count() ? kSmemLimit / 2 - 1024 : kSmemLimit;
     int stages = (int)((budget - fixed) / stage);
     stages = stages < 12 ? stages : 12;
     stages = stages < per_cta ? stages : per_cta;
@@ -669,34 +670,55 @@ int pairs_launch(const Int8Args& a, int bn, cudaStream_t st) {
     return check_launch("linear_int8_pairs_kernel");
 }
 
-}  // namespace
-
-int linear_int8_tiles(const Int8Args& a, cudaStream_t st) {
-    // the token tile that holds the rows, 128 at most; K split until the SMs
-    // each have a CTA, at least two K blocks each
-    const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
-    const int64_t ctas = (int64_t)ceil_div(a.cols, 128) * ceil_div(a.rows, bn);
-    const int k_blocks = ceil_div(a.K, kBlockK);
-    int split = 1;
-    while (split < 8 && split < bn / 4 && ctas * split < sm_count() && k_blocks >= 4 * split) split *= 2;
-    int status = F2S_OK;
-    F2S_DTYPE_SWITCH(a.dtype, switch (bn) {
-        case 16: status = tiles_launch<T, 16>(a, split, st); break;
-        case 32: status = tiles_launch<T, 32>(a, split, st); break;
-        case 64: status = tiles_launch<T, 64>(a, split, st); break;
-        default: status = tiles_launch<T, 128>(a, split, st); break;
-    });
-    return status;
+// The forms' times on a B200, in us, fitted to 60 shapes of 1 to 2,048 tokens: a
+// CTA of `tiles` takes 3 and 0.45 per K block and the kernel 2 around that; joining
+// K parts takes up to 0.6 with the tokens, and clusters of 4 and 8 leave some SMs
+// without a CTA (a GPU processing cluster holds whole ones). `pairs` takes 5.5 and
+// 0.38 per K block of each 256 x bn tile.
+float tiles_time(const Int8Args& a, int bn, int split) {
+    const int64_t ctas = (int64_t)ceil_div(a.cols, 128) * ceil_div(a.rows, bn) * split;
+    const int sms = sm_count(), usable = split == 8 ? sms * 7 / 10 : split == 4 ? sms * 9 / 10 : sms;
+    return 2.0f + (split > 1 ? 0.6f * (float)bn / 64.0f : 0.0f) +
+           (float)ceil_div64(ctas, usable) * (3.0f + 0.45f * (float)ceil_div(ceil_div(a.K, kBlockK), split));
 }
 
-int linear_int8_pairs(const Int8Args& a, cudaStream_t st) {
-    // the channel tile with the fewest columns computed (one of 64 takes as
-    // long as one of 128), the larger on ties
+int tile_tokens(const Int8Args& a) { return a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : 64; }
+
+int tile_split(const Int8Args& a, int bn) {
+    int split = 1;
+    for (int s = 2; s <= 8 && s <= ceil_div(a.K, kBlockK); s *= 2)
+        if (tiles_time(a, bn, s) < tiles_time(a, bn, split)) split = s;
+    return split;
+}
+
+// The channel tile with the fewest columns computed (one of 64 takes as long as
+// one of 128), the larger on ties.
+int pair_channels(const Int8Args& a) {
     int bn = 256;
     for (int c : {192, 128, 64})
         if (ceil_div(a.cols, c) * (c < 128 ? 128 : c) < ceil_div(a.cols, bn) * bn) bn = c;
+    return bn;
+}
+
+float pairs_time(const Int8Args& a, int bn) {
+    const int64_t tiles = (int64_t)ceil_div(a.rows, 256) * ceil_div(a.cols, bn);
+    return 5.5f + 0.38f * (float)ceil_div64(tiles, sm_count() / 2) * (float)ceil_div(a.K, kBlockK);
+}
+
+}  // namespace
+
+int linear_int8_tensor(const Int8Args& a, cudaStream_t st) {
+    const int bn = tile_tokens(a), split = tile_split(a, bn), channels = pair_channels(a);
     int status = F2S_OK;
-    F2S_DTYPE_SWITCH(a.dtype, status = pairs_launch<T>(a, bn, st));
+    if (pairs_time(a, channels) < tiles_time(a, bn, split)) {
+        F2S_DTYPE_SWITCH(a.dtype, status = pairs_launch<T>(a, channels, st));
+        return status;
+    }
+    F2S_DTYPE_SWITCH(a.dtype, switch (bn) {
+        case 16: status = tiles_launch<T, 16>(a, split, st); break;
+        case 32: status = tiles_launch<T, 32>(a, split, st); break;
+        default: status = tiles_launch<T, 64>(a, split, st); break;
+    });
     return status;
 }
 

@@ -1,5 +1,4 @@
-// The 8-bit product's operands and its two tensor-core forms (linear_int8.cu
-// chooses).
+// The 8-bit product's operands and its tensor-core forms.
 #pragma once
 
 #include "common.cuh"
@@ -20,8 +19,7 @@ struct Int8Args {
     int rows, cols, K;
 };
 
-// x and w 16-byte aligned with pitches of multiples of 16.
-int linear_int8_tiles(const Int8Args& g, cudaStream_t st);  // 128 channels x up to 128 tokens, K split
-int linear_int8_pairs(const Int8Args& g, cudaStream_t st);  // 256 x 256 tiles by CTA pairs
+// On tcgen05: x and w 16-byte aligned with pitches of multiples of 16.
+int linear_int8_tensor(const Int8Args& g, cudaStream_t st);
 
 }  // namespace f2s

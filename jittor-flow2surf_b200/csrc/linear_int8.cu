@@ -1,7 +1,6 @@
 // Product of 8-bit integer rows with scales for each token and channel:
 //   y[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k] + b[n],
 // the sum exact in 32 bits (K <= 131,071 keeps 2^14 K below 2^31).
-#include <stdlib.h>
 #include "gemm_int8.cuh"
 #include "row_ops.cuh"
 
@@ -16,8 +15,14 @@ constexpr int kMaxK = 131071;
 // channels (and 1 / kSplit of their K, joined in shared memory), 16 bytes of
 // each per lane and step, four products and sums per dp4a; its loads of several
 // steps are in flight at once.
-constexpr int kFew = 8;        // tokens at most
-constexpr int kFewWarps = 8;   // per block
+//
+// Against the tensor cores, which take 4.5 us at least and little more for more
+// tokens (both in us):   1 x 4096 -> 4096 6.2, 7.5;   4 x 192 -> 1536 3.1, 4.2;
+// 4 x 8192 -> 1024 4.4, 7.2;   4 x 4096 -> 4096 9.7, 8.0;   1 x 8192 -> 8192 18.6,
+// 17.8: past 2^25 products of 8-bit values this form's arithmetic costs more.
+constexpr int kFew = 4;  // tokens at most
+constexpr int64_t kFewProducts = 1 << 25;
+constexpr int kFewWarps = 8;  // per block
 
 template <typename T, int R>
 __global__ void __launch_bounds__(32 * kFewWarps) linear_int8_few_kernel(const Int8Args g, int split) {
@@ -81,8 +86,7 @@ int few_launch(const Int8Args& g, cudaStream_t st) {
     auto go = [&](auto kernel) { kernel<<<blocks, 32 * kFewWarps, 0, st>>>(g, split); };
     if (g.rows == 1) go(linear_int8_few_kernel<T, 1>);
     else if (g.rows == 2) go(linear_int8_few_kernel<T, 2>);
-    else if (g.rows <= 4) go(linear_int8_few_kernel<T, 4>);
-    else go(linear_int8_few_kernel<T, 8>);
+    else go(linear_int8_few_kernel<T, 4>);
     return check_launch("linear_int8_few_kernel");
 }
 
@@ -156,19 +160,11 @@ extern "C" int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scal
     cudaStream_t st = f2s::as_stream(stream);
     f2s::TraceScope trace(f2s::kTagGemmInt8, st);
     using f2s::rows::aligned16;
-    if (aligned16(x) && aligned16(w) && (ldx % 16 == 0 || rows == 1) && (ldw % 16 == 0 || cols == 1))
-    {
-        const char* form = getenv("F2S_FORM");
-        if (form && *form == 't') return f2s::linear_int8_tiles(g, st);
-        if (form && *form == 'p') return f2s::linear_int8_pairs(g, st);
-        if ((form && *form == 'f') || (!form && rows <= 4)) {
-            int status = F2S_OK;
-            F2S_DTYPE_SWITCH(dtype, status = f2s::few_launch<T>(g, st));
-            return status;
-        }
-        return rows >= 1024 ? f2s::linear_int8_pairs(g, st) : f2s::linear_int8_tiles(g, st);
-    }
+    const bool aligned = aligned16(x) && aligned16(w) && (ldx % 16 == 0 || rows == 1) && (ldw % 16 == 0 || cols == 1);
+    if (aligned && !(rows <= f2s::kFew && (int64_t)rows * cols * K <= f2s::kFewProducts))
+        return f2s::linear_int8_tensor(g, st);
     int status = F2S_OK;
-    F2S_DTYPE_SWITCH(dtype, status = f2s::any_launch<T>(g, st));
+    if (aligned) F2S_DTYPE_SWITCH(dtype, status = f2s::few_launch<T>(g, st))
+    else F2S_DTYPE_SWITCH(dtype, status = f2s::any_launch<T>(g, st));
     return status;
 }
