@@ -43,7 +43,7 @@ __device__ __forceinline__ float reciprocal_rms(float sum, int C, float eps) {
 // k8: 8-bit rows. The products s w of a 16-bit type are exact in fp32; those of
 // fp32 are taken in 64 bits for the maximum and at rounding borders.
 template <typename T, int E, int TPR, bool kWide, bool k8>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, 2 * sizeof(T)))
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, 2 * (kWide ? sizeof(T) : 4)))
 add_rms_norm_kernel(const NormArgs g) {
     using S = Slice<T, E, TPR, kWide>;
     constexpr bool kExact64 = k8 && sizeof(T) == 4;
@@ -146,7 +146,7 @@ int norm_launch(const NormArgs& g, int dtype, cudaStream_t st) {
     const bool wide = g.C % vec == 0 && aligned16(g.x) && (g.ldx % vec == 0 || g.nrows == 1) && aligned16(g.weight) &&
                       (!g.residual || (aligned16(g.residual) && (g.ldr % vec == 0 || g.nrows == 1) && aligned16(g.stream))) &&
                       (k8 ? (aligned16(g.q) && (g.ldq % vec == 0 || g.nrows == 1)) : aligned16(g.y));
-    const Shape s = pick_shape(kForward, size, g.nrows, g.C, wide);
+    const Shape s = pick_shape(kForward, held_size(size, wide), g.nrows, g.C, wide);
     const int64_t blocks = ceil_div64(g.nrows, block_rows(s.tpr));
     F2S_LIMIT(blocks <= INT32_MAX, "add_rms_norm: %lld rows", (long long)g.nrows);
     TraceScope trace(kTagRmsNorm, st);
@@ -187,7 +187,7 @@ constexpr int grad_resident(int tpr, int E, int size) {
 }
 
 template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, grad_resident(TPR, E, sizeof(T)))
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, grad_resident(TPR, E, kWide ? sizeof(T) : 4))
 add_rms_norm_grad_kernel(const NormGradArgs g) {
     using S = Slice<T, E, TPR, kWide>;
     constexpr int kRows = TPR <= 32 ? 256 / TPR : 1;
@@ -199,8 +199,8 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
     for (int i = 0; i < E; ++i) dw[i] = 0.0f;
     // Rows of one warp or less: the other warps' loads hide a row's latency.
     // Rows of a block: its warps wait for one another, so the next row is on
-    // its way meanwhile.
-    constexpr bool kAhead = TPR > 32;
+    // its way meanwhile (single values have no registers for that).
+    constexpr bool kAhead = TPR > 32 && kWide;
     Held<T, E, kWide> w, s, dy, ds, s_next, dy_next, ds_next;
     load_held<S>(static_cast<const T*>(g.weight), g.C, t, w);
     auto fetch = [&](int64_t row) {
@@ -334,9 +334,9 @@ void weight_grad_launch(const float* partial, int blocks, int C, void* dw, cudaS
 
 // Blocks of the backward: those that are resident at one time, each with
 // several rows to share its dw over.
-int grad_blocks(int64_t nrows, const Shape& s, int dtype) {
+int grad_blocks(int64_t nrows, const Shape& s, int size) {
     const int64_t all = ceil_div64(nrows, block_rows(s.tpr));
-    const int64_t most = (int64_t)sm_count() * grad_resident(s.tpr, s.e, dtype_size(dtype));
+    const int64_t most = (int64_t)sm_count() * grad_resident(s.tpr, s.e, size);
     return (int)(all < most ? all : most);
 }
 
@@ -345,7 +345,8 @@ size_t grad_workspace(int64_t nrows, int C) {
     int blocks = 0;
     for (int dtype : {F2S_DTYPE_F32, F2S_DTYPE_BF16})
         for (bool wide : {false, true}) {
-            const int b = grad_blocks(nrows, pick_shape(kGrad, dtype_size(dtype), nrows, C, wide), dtype);
+            const int size = held_size(dtype_size(dtype), wide);
+            const int b = grad_blocks(nrows, pick_shape(kGrad, size, nrows, C, wide), size);
             blocks = b > blocks ? b : blocks;
         }
     return (size_t)blocks * C * sizeof(float);
@@ -413,8 +414,9 @@ extern "C" int f2s_add_rms_norm_backward(const void* s, int64_t lds, const void*
     const bool wide = C % vec == 0 && pitched(s, lds) && pitched(dy, lddy) && (!ds || pitched(ds, ldds)) &&
                       aligned16(weight) && aligned16(dx);
     NormGradArgs g{s, lds, weight, dy, lddy, ds, ldds, rows, C, eps, dx, dweight ? static_cast<float*>(workspace) : nullptr};
-    const Shape shape = pick_shape(kGrad, dtype_size(dtype), rows, C, wide);
-    const int blocks = grad_blocks(rows, shape, dtype);
+    const int size = held_size(dtype_size(dtype), wide);
+    const Shape shape = pick_shape(kGrad, size, rows, C, wide);
+    const int blocks = grad_blocks(rows, shape, size);
     TraceScope trace(kTagRmsNorm, st);
     F2S_DTYPE_SWITCH(dtype, dispatch<kGrad, sizeof(T)>(shape, wide, [&](auto e, auto tpr, auto w) {
         add_rms_norm_grad_kernel<T, e.value, tpr.value, w.value><<<blocks, block_threads(tpr.value), 0, st>>>(g);

@@ -399,6 +399,9 @@ constexpr int most_channels(Kind kind, int size, int tpr) {
 }
 constexpr int kThreads[] = {8, 32, 128, 256, 512, 1024};
 
+// Single values of a 16-bit type are held in fp32.
+constexpr int held_size(int size, bool wide) { return wide ? size : 4; }
+
 // (TPR, E) for a row of C channels: the fewest threads that hold it, since each
 // thread's share of the reduction and of the row's constants costs as much as
 // ten channels, and then the fewest registers. Rows past 512 x most_channels
@@ -413,10 +416,12 @@ inline Shape pick_shape(Kind kind, int size, int64_t nrows, int C, bool wide) {
     int i = 0;
     while (i < 4 && kThreads[i] * most_channels(kind, size, kThreads[i]) < C) ++i;
     while (i < 4 && C > kThreads[i] * 8 && nrows * kThreads[i] < (int64_t)sm_count() * 512) ++i;
-    if (kThreads[i] * 32 < C) i = 5;
+    // single values: 8, 16 or 32; the backward's on 1,024 threads before they spill
+    // (8,192 x 4,097: 210 us against 466; the forward 157 against 110)
+    if (kThreads[i] * 32 < C || (!wide && kind == kGrad && i == 4 && C > 512 * 8)) i = 5;
     const int e = ceil_div(ceil_div(C, kThreads[i]), 8) * 8;
-    // single values: 8, 16 or 32; 1,024 threads: 32
-    return {kThreads[i], i == 5 || (!wide && e > 16) ? 32 : e};
+    const bool all = i == 5 && (wide || kind == kForward);
+    return {kThreads[i], all || (!wide && e > 16) ? 32 : e};
 }
 
 // Blocks of `threads` per SM that E channels held in `size` bytes each leave
@@ -434,23 +439,27 @@ using Const = std::integral_constant<int, kValue>;
 
 template <Kind kKind, int kSize, int kTpr, typename F>
 void dispatch_channels(const Shape& s, bool wide, F f) {
-    constexpr int most = kTpr == 512 ? 32 : most_channels(kKind, kSize, kTpr);
-    if constexpr (kTpr == 1024) {
-        wide ? f(Const<32>(), Const<kTpr>(), std::true_type()) : f(Const<32>(), Const<kTpr>(), std::false_type());
+    constexpr int most = kTpr >= 512 ? 32 : most_channels(kKind, kSize, kTpr);
+    constexpr int most_single = kTpr == 1024 || (kTpr == 512 && kKind == kForward) ? 32 : most_channels(kKind, 4, kTpr);
+    if (!wide) {
+        constexpr bool few = kTpr < 1024 || kKind == kGrad;  // a forward of 1,024 threads takes 32
+        if constexpr (few)
+            if (s.e == 8) f(Const<8>(), Const<kTpr>(), std::false_type());
+        if constexpr (few && most_single >= 16)
+            if (s.e == 16) f(Const<16>(), Const<kTpr>(), std::false_type());
+        if constexpr (most_single >= 32)
+            if (s.e == 32) f(Const<32>(), Const<kTpr>(), std::false_type());
         return;
     }
-    if (s.e == 8) wide ? f(Const<8>(), Const<kTpr>(), std::true_type()) : f(Const<8>(), Const<kTpr>(), std::false_type());
-    if constexpr (most >= 16)
-        if (s.e == 16)
-            wide ? f(Const<16>(), Const<kTpr>(), std::true_type()) : f(Const<16>(), Const<kTpr>(), std::false_type());
-    if constexpr (most >= 24)
-        if (s.e == 24 && wide) f(Const<24>(), Const<kTpr>(), std::true_type());
-    if constexpr (most >= 24)  // single values of 24 channels take the kernel of 32
-        if (s.e == 32 && (most >= 32 || !wide)) {
-            if constexpr (most >= 32)
-                if (wide) f(Const<32>(), Const<kTpr>(), std::true_type());
-            if (!wide) f(Const<32>(), Const<kTpr>(), std::false_type());
-        }
+    if constexpr (kTpr < 1024) {
+        if (s.e == 8) f(Const<8>(), Const<kTpr>(), std::true_type());
+        if constexpr (most >= 16)
+            if (s.e == 16) f(Const<16>(), Const<kTpr>(), std::true_type());
+        if constexpr (most >= 24)
+            if (s.e == 24) f(Const<24>(), Const<kTpr>(), std::true_type());
+    }
+    if constexpr (most >= 32)
+        if (s.e == 32) f(Const<32>(), Const<kTpr>(), std::true_type());
 }
 
 // f(E, TPR, wide) for the shape, as integral constants.

@@ -10,7 +10,7 @@ namespace {
 using namespace rows;
 
 template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, sizeof(T)))
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, kWide ? sizeof(T) : 4))
 quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t nrows, int width, int8_t* __restrict__ q8,
                      int64_t ldq, float* __restrict__ scale) {
     using S = Slice<T, E, TPR, kWide>;
@@ -41,31 +41,48 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t nrows, int wi
     if (live && t == 0) scale[row] = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
 }
 
-// y = scale q. kWide: 16 channels per thread (one 16-byte load); else one.
-template <typename T, bool kWide>
+// y = scale q, 16 channels (one 16-byte load) per thread.
+template <typename T>
 __global__ void __launch_bounds__(256)
-dequantize_rows_kernel(const int8_t* __restrict__ q8, int64_t ldq, const float* __restrict__ scale, int width,
-                       int per_row, int64_t items, T* __restrict__ y, int64_t ldy) {
+dequantize_rows_kernel(const int8_t* __restrict__ q8, int64_t ldq, const float* __restrict__ scale, int per_row,
+                       int64_t items, T* __restrict__ y, int64_t ldy) {
     const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (item >= items) return;
     const int64_t row = items <= INT32_MAX ? (int64_t)((uint32_t)item / (uint32_t)per_row) : item / per_row;
-    const int c = (int)(item - row * per_row) * (kWide ? 16 : 1);
+    const int c = (int)(item - row * per_row) * 16;
     const float s = scale[row];
-    if constexpr (kWide) {
-        const uint4 u = *reinterpret_cast<const uint4*>(q8 + row * ldq + c);
-        float v[16];
-        widen8(u.x, v);
-        widen8(u.y, v + 4);
-        widen8(u.z, v + 8);
-        widen8(u.w, v + 12);
+    const uint4 u = *reinterpret_cast<const uint4*>(q8 + row * ldq + c);
+    float v[16];
+    widen8(u.x, v);
+    widen8(u.y, v + 4);
+    widen8(u.z, v + 8);
+    widen8(u.w, v + 12);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= s;
-        uint4* to = reinterpret_cast<uint4*>(y + row * ldy + c);
+    for (int i = 0; i < 16; ++i) v[i] *= s;
+    uint4* to = reinterpret_cast<uint4*>(y + row * ldy + c);
 #pragma unroll
-        for (int i = 0; i < 16 / kVec<T>; ++i) to[i] = pack16<T>(v + i * kVec<T>);
-    } else {
-        y[row * ldy + c] = from_f32<T>((float)q8[row * ldq + c] * s);
-    }
+    for (int i = 0; i < 16 / kVec<T>; ++i) to[i] = pack16<T>(v + i * kVec<T>);
+}
+
+// The same for any pitch and width: a warp takes 256 channels of a row, eight
+// per lane, 32 apart.
+template <typename T>
+__global__ void __launch_bounds__(256)
+dequantize_any_kernel(const int8_t* __restrict__ q8, int64_t ldq, const float* __restrict__ scale, int width,
+                      int per_row, int64_t items, T* __restrict__ y, int64_t ldy) {
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (item >= items) return;
+    const int64_t row = items <= INT32_MAX ? (int64_t)((uint32_t)item / (uint32_t)per_row) : item / per_row;
+    const int c = (int)(item - row * per_row) * 256 + (threadIdx.x & 31);
+    const int8_t* from = q8 + row * ldq + c;
+    T* to = y + row * ldy + c;
+    const float s = scale[row];
+    int v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + 32 * i < width ? from[32 * i] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (c + 32 * i < width) to[32 * i] = from_f32<T>((float)v[i] * s);
 }
 
 template <typename T>
@@ -74,7 +91,7 @@ int quantize_launch(const void* x, int64_t ldx, int64_t nrows, int C, int8_t* q,
     constexpr int vec = kVec<T>;
     const bool wide = C % vec == 0 && aligned16(x) && aligned16(q) &&
                       ((ldx % vec == 0 && ldq % vec == 0) || nrows == 1);
-    const Shape s = pick_shape(kForward, sizeof(T), nrows, C, wide);
+    const Shape s = pick_shape(kForward, held_size(sizeof(T), wide), nrows, C, wide);
     const int64_t blocks = ceil_div64(nrows, block_rows(s.tpr));
     F2S_LIMIT(blocks <= INT32_MAX, "quantize_rows: %lld rows", (long long)nrows);
     TraceScope trace(kTagRows8, st);
@@ -90,16 +107,13 @@ int dequantize_launch(const int8_t* q, int64_t ldq, const float* scale, int64_t 
                       cudaStream_t st) {
     const bool wide = C % 16 == 0 && aligned16(q) && aligned16(y) &&
                       ((ldq % 16 == 0 && ldy % kVec<T> == 0) || nrows == 1);
-    const int per_row = wide ? C / 16 : C;
-    const int64_t items = nrows * per_row, blocks = ceil_div64(items, 256);
+    const int per_row = wide ? C / 16 : ceil_div(C, 256);
+    const int64_t items = nrows * per_row, blocks = ceil_div64(items, wide ? 256 : 8);
     F2S_LIMIT(blocks <= INT32_MAX, "dequantize_rows: %lld rows of %d", (long long)nrows, C);
     TraceScope trace(kTagRows8, st);
-    if (wide)
-        dequantize_rows_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(q, ldq, scale, C, per_row, items,
-                                                                          static_cast<T*>(y), ldy);
-    else
-        dequantize_rows_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(q, ldq, scale, C, per_row, items,
-                                                                           static_cast<T*>(y), ldy);
+    T* to = static_cast<T*>(y);
+    if (wide) dequantize_rows_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(q, ldq, scale, per_row, items, to, ldy);
+    else dequantize_any_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(q, ldq, scale, C, per_row, items, to, ldy);
     return check_launch("dequantize_rows_kernel");
 }
 
