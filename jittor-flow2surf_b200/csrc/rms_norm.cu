@@ -179,15 +179,15 @@ struct NormGradArgs {
     float* partial;  // (blocks, C), or null: no weight gradient
 };
 
-// Blocks per SM: 1,024 threads with 8 16-bit channels each (64 registers), 512
-// with more (128).
-constexpr int grad_resident(int tpr, int E, int size) {
-    const int threads = E * size <= 16 ? 1024 : 512;
+// Blocks per SM: 1,024 threads with 8 16-bit or 8 single channels each (64
+// registers), 512 with more (128).
+constexpr int grad_resident(int tpr, int E, int size, bool wide) {
+    const int threads = E * size <= 16 || (!wide && E == 8) ? 1024 : 512;
     return threads / block_threads(tpr) > 0 ? threads / block_threads(tpr) : 1;
 }
 
 template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, grad_resident(TPR, E, kWide ? sizeof(T) : 4))
+__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, grad_resident(TPR, E, held_size(sizeof(T), kWide), kWide))
 add_rms_norm_grad_kernel(const NormGradArgs g) {
     using S = Slice<T, E, TPR, kWide>;
     constexpr int kRows = TPR <= 32 ? 256 / TPR : 1;
@@ -334,9 +334,9 @@ void weight_grad_launch(const float* partial, int blocks, int C, void* dw, cudaS
 
 // Blocks of the backward: those that are resident at one time, each with
 // several rows to share its dw over.
-int grad_blocks(int64_t nrows, const Shape& s, int size) {
+int grad_blocks(int64_t nrows, const Shape& s, int size, bool wide) {
     const int64_t all = ceil_div64(nrows, block_rows(s.tpr));
-    const int64_t most = (int64_t)sm_count() * grad_resident(s.tpr, s.e, size);
+    const int64_t most = (int64_t)sm_count() * grad_resident(s.tpr, s.e, size, wide);
     return (int)(all < most ? all : most);
 }
 
@@ -346,7 +346,7 @@ size_t grad_workspace(int64_t nrows, int C) {
     for (int dtype : {F2S_DTYPE_F32, F2S_DTYPE_BF16})
         for (bool wide : {false, true}) {
             const int size = held_size(dtype_size(dtype), wide);
-            const int b = grad_blocks(nrows, pick_shape(kGrad, size, nrows, C, wide), size);
+            const int b = grad_blocks(nrows, pick_shape(kGrad, size, nrows, C, wide), size, wide);
             blocks = b > blocks ? b : blocks;
         }
     return (size_t)blocks * C * sizeof(float);
@@ -416,7 +416,7 @@ extern "C" int f2s_add_rms_norm_backward(const void* s, int64_t lds, const void*
     NormGradArgs g{s, lds, weight, dy, lddy, ds, ldds, rows, C, eps, dx, dweight ? static_cast<float*>(workspace) : nullptr};
     const int size = held_size(dtype_size(dtype), wide);
     const Shape shape = pick_shape(kGrad, size, rows, C, wide);
-    const int blocks = grad_blocks(rows, shape, size);
+    const int blocks = grad_blocks(rows, shape, size, wide);
     TraceScope trace(kTagRmsNorm, st);
     F2S_DTYPE_SWITCH(dtype, dispatch<kGrad, sizeof(T)>(shape, wide, [&](auto e, auto tpr, auto w) {
         add_rms_norm_grad_kernel<T, e.value, tpr.value, w.value><<<blocks, block_threads(tpr.value), 0, st>>>(g);
