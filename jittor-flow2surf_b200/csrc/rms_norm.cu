@@ -115,12 +115,14 @@ add_rms_norm_kernel(const NormArgs g) {
             for (int j = 0; j < 8; ++j) a[j] *= b[j];
             if constexpr (kExact64) {
                 // `from` holds the stream: x, or this thread's own channels of it
-                store8_chunk<S, kWide>(g.q + at * g.ldq, C, t, i, a, rounding, [&](int j) {
+                store8_chunk<false, S, kWide>(g.q + at * g.ldq, C, t, i, a, rounding, [&](int j) {
                     const int c = S::channel(i + j, t);
                     return c < C ? (double)from[c] * (double)weight[c] * (double)rounding.scale : 0.0;
                 });
             } else {
-                store8_chunk<S, kWide>(g.q + at * g.ldq, C, t, i, a, rounding, [&](int j) { return a[j]; });
+                // products of bf16 have 16 bits, of fp16 22
+                store8_chunk<std::is_same<T, __nv_bfloat16>::value, S, kWide>(
+                    g.q + at * g.ldq, C, t, i, a, rounding, [&](int j) { return a[j]; });
             }
         }
         if (live && t == 0)

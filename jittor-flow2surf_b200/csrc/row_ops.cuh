@@ -249,9 +249,14 @@ __device__ __forceinline__ void row_sum_max(float& a, M& m, float* shared_a, M* 
 // inv = 127 / m is off by at most 127 (2^-23 + 2^-24 of inv, 2^-24 of a rounded
 // v, 2^-24 of a rounded m) = 3.8e-5, so the nearest whole number of t is the
 // answer unless t lies next to a half, past kBorder. There the sign of
-// 254 v - c m with c / 2 that half decides, taken without rounding. (One value in
-// 10,000, but more where v and m have few bits: the quotients of bf16 values
-// are exact halves about once in 1,000.)
+// 254 v - c m with c / 2 that half decides, taken without rounding (one value in
+// 10,000).
+// Where v and m have at most 16 bits (kShort) there is no such case to look at,
+// although exact halves are common then (about one quotient of bf16 values in
+// 1,000, which cost SwiGLU's forward a quarter of its instructions): one step
+// with the exact remainder makes t the rounded quotient itself, exact where that
+// is a half, and every other quotient is 2^-17 from a half or more, the rounding's
+// error 2^-18 or less.
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
 constexpr float kBorder = 0.49995f;
 // Below 1e-30, 127 / m may overflow and products lose bits, and above 1e30
@@ -282,6 +287,7 @@ template <typename M>
 struct Rounding {
     M m;          // scaled
     float inv;    // 127 / m
+    float reciprocal;  // 1 / m
     float scale;  // of the row's values, 1 unless `odd`
     bool odd;     // a tiny, huge, zero or not finite row
     bool zero;    // a row of zeros, or one that is not finite
@@ -293,7 +299,8 @@ struct Rounding {
             scale = mf < kTiny ? kScaleTiny : kScaleHuge;
             m *= (M)scale;
         }
-        inv = zero ? 0.0f : 127.0f * f2s_rcp_approx((float)m);
+        reciprocal = zero ? 0.0f : f2s_rcp_approx((float)m);
+        inv = 127.0f * reciprocal;
     }
 };
 
@@ -312,13 +319,41 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // 8 values of a thread to 8 bits, in the low bytes of q; at(j): value j in m's
 // type.
-template <typename M, typename F>
+template <bool kShort, typename M, typename F>
 __device__ __forceinline__ void round8(float (&v)[8], const Rounding<M>& r, uint32_t (&q)[8], F at) {
     if (r.odd) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= r.scale;
+    }
+    if constexpr (kShort) {
+        const uint64_t top = pair(127.0f, 127.0f), by = pair(r.reciprocal, r.reciprocal),
+                       minus_m = pair(-(float)r.m, -(float)r.m), magic = pair(kMagic, kMagic);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const uint64_t a = mul2(pair(v[j], v[j + 1]), top), t = mul2(a, by);
+            float s0, s1;
+            unpair(add2(fma2(fma2(t, minus_m, a), by, t), magic), s0, s1);
+            q[j] = __float_as_uint(s0);
+            q[j + 1] = __float_as_uint(s1);
+        }
+        if (r.zero) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = 0u;
+        }
+        return;
     }
     float off = 0.0f;
     const uint64_t inv = pair(r.inv, r.inv), magic = pair(kMagic, kMagic), minus = pair(-1.0f, -1.0f);
@@ -355,11 +390,11 @@ __device__ __forceinline__ void round8(float (&v)[8], const Rounding<M>& r, uint
 
 // Chunk i of a thread's channels, v, to 8 bits in `row` (of a pitch that keeps
 // vectors aligned where kWide). at(j): value j of the chunk in m's type, scaled.
-template <typename S, bool kWide, typename M, typename F>
+template <bool kShort, typename S, bool kWide, typename M, typename F>
 __device__ __forceinline__ void store8_chunk(int8_t* row, int C, int t, int i, float (&v)[8], const Rounding<M>& r,
                                              F at) {
     uint32_t q[8];
-    round8(v, r, q, at);
+    round8<kShort>(v, r, q, at);
     const int c = S::channel(i, t);
     if constexpr (kWide && S::V == 8) {
         if (c < C)

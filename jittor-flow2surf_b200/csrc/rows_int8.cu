@@ -36,7 +36,7 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t nrows, int wi
     for (int i = 0; i < E; i += 8) {
         float v[8];
         held.get(i, v);
-        store8_chunk<S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
+        store8_chunk<sizeof(T) == 2, S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
     }
     if (live && t == 0) scale[row] = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
 }

@@ -83,6 +83,7 @@ __device__ __forceinline__ void store_group(T* row, int lane, int left, const fl
 
 // One group's checkpoint: thread `lane` keeps its 16 channels, in its own
 // order, as 16 consecutive bytes.
+template <bool kShort>
 __device__ __forceinline__ void keep_group(const float (&v)[kEach], int lane, int8_t* q8, float* scale) {
     float m = 0.0f;
 #pragma unroll
@@ -96,7 +97,7 @@ __device__ __forceinline__ void keep_group(const float (&v)[kEach], int lane, in
         uint32_t q[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) held[j] = v[i + j];
-        round8(held, rounding, q, [&](int j) { return held[j]; });
+        round8<kShort>(held, rounding, q, [&](int j) { return held[j]; });
         w[i / 4] = pack_bytes(q[0], q[1], q[2], q[3]);
         w[i / 4 + 1] = pack_bytes(q[4], q[5], q[6], q[7]);
     }
@@ -128,8 +129,8 @@ swiglu_kernel(const T* __restrict__ projected, int64_t ld, int H, int groups, in
     store_group<T, kForm>(y + row * (int64_t)H + first, lane, left, h);
     if constexpr (kKeep) {
         // the shuffles need every lane of the warp, live or not
-        keep_group(g, lane, live ? kept + u * (2 * kGroup) : nullptr, scales + 2 * u);
-        keep_group(v, lane, live ? kept + u * (2 * kGroup) + kGroup : nullptr, scales + 2 * u + 1);
+        keep_group<sizeof(T) == 2>(g, lane, live ? kept + u * (2 * kGroup) : nullptr, scales + 2 * u);
+        keep_group<sizeof(T) == 2>(v, lane, live ? kept + u * (2 * kGroup) + kGroup : nullptr, scales + 2 * u + 1);
     }
 }
 
@@ -219,7 +220,7 @@ swiglu_int8_kernel(const T* __restrict__ projected, int64_t ld, int64_t nrows, i
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = h[i + j];
-        store8_chunk<S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
+        store8_chunk<false, S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
     }
     if (live && t == 0) scale[row] = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
 }
