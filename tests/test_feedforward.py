@@ -383,6 +383,39 @@ def test_quantize_rows_at_borders(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_16_bit_value_against_many_maxima(cuda, dtype):
+    """All positive values of the binades in which 127 v / m is between 1/4 and
+    127, for maxima of every kind of significand: exact halves are common here."""
+    bits = 7 if dtype == torch.bfloat16 else 10
+    significands = torch.arange(2**bits, 2 ** (bits + 1), dtype=torch.float64)
+    values = torch.cat([significands * 2.0**e for e in range(-10, 1)]) * 2.0**-bits  # below 2
+    step = 1 if dtype == torch.bfloat16 else 5
+    maxima = significands[::step] * 2.0**-bits
+    x = torch.where(values <= maxima[:, None], values, 0.0)
+    x = torch.cat([maxima[:, None], x, -x], 1).to(dtype).to(cuda)
+    want = nearest_whole(x.double(), row_max(x.double()))
+    assert torch.equal(f2s.quantize_rows(x).values, want)
+    # as a norm's products, and as a checkpoint group's values
+    one = torch.ones(x.shape[1], dtype=dtype, device=cuda)
+    assert torch.equal(f2s.add_rms_norm_int8(x, one)[0].values, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_norm_int8_of_products_at_halves(cuda, dtype):
+    """Streams and weights of few bits, whose products make 127 p / m an exact
+    half often; each row's largest product is another."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randint(-255, 256, (400, 2048), generator=g).to(dtype).to(cuda)
+    w = torch.randint(1, 256, (2048,), generator=g).to(dtype).to(cuda)
+    p = x.double() * w.double()
+    twice = 254 * p / row_max(p)
+    assert ((twice == twice.round()) & (twice.remainder(2) == 1)).sum() > 100  # halves are there
+    assert torch.equal(f2s.add_rms_norm_int8(x, w)[0].values, nearest_whole(p, row_max(p)))
+
+
+@pytest.mark.gpu
 def test_shapes_without_rows_and_of_any_rank(cuda):
     x = normal(2, 3, 5, 40, seed=1).to(cuda)
     eight = f2s.quantize_rows(x)
