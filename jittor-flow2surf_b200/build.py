@@ -70,31 +70,44 @@ def _compile(src: Path, force: bool, extra: list[str]) -> tuple[Path, str]:
     return obj, proc.stderr
 
 
-def _build_binding(force: bool) -> None:
-    """The PyTorch binding, against the torch of this interpreter (a stamp in
-    _build/ names its version)."""
+def _compile_binding(force: bool) -> tuple[Path, str]:
+    """Object of the PyTorch binding, against the torch of this interpreter (a
+    stamp beside it names their versions)."""
     import torch
 
-    stamp = BUILD / "feedforward_torch.stamp"
+    obj, stamp = BUILD / "feedforward_torch.o", BUILD / "feedforward_torch.stamp"
     wanted = f"{torch.__version__} {sys.version}"
-    inputs = [BINDING_SOURCE, *INCLUDE.glob("*.h")]
-    if (not force and BINDING.exists() and stamp.exists() and stamp.read_text() == wanted
-            and BINDING.stat().st_mtime >= max(i.stat().st_mtime for i in inputs)):
-        return
+    newest = max(i.stat().st_mtime for i in (BINDING_SOURCE, *INCLUDE.glob("*.h")))
+    if (not force and obj.exists() and stamp.exists() and stamp.read_text() == wanted
+            and obj.stat().st_mtime >= newest):
+        return obj, ""
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{INCLUDE}", "-isystem", str(root / "include"),
            "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
-           str(BINDING_SOURCE), "-o", str(BINDING), f"-L{LIBRARY.parent}", f"-l:{LIBRARY.name}",
-           "-Wl,-rpath,$ORIGIN", f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
-           "-lc10", "-lc10_cuda"]
+           "-c", str(BINDING_SOURCE), "-o", str(obj)]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"{cmd[0]} failed for {BINDING_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
+        raise RuntimeError(f"g++ failed for {BINDING_SOURCE.name}:\n{proc.stdout}\n{proc.stderr}")
     stamp.write_text(wanted)
+    return obj, proc.stderr
+
+
+def _link_binding(obj: Path, force: bool) -> None:
+    import torch
+
+    if not force and BINDING.exists() and BINDING.stat().st_mtime >= obj.stat().st_mtime:
+        return
+    libraries = Path(torch.__file__).resolve().parent / "lib"
+    cmd = ["g++", "-shared", str(obj), "-o", str(BINDING), f"-L{LIBRARY.parent}",
+           f"-l:{LIBRARY.name}", "-Wl,-rpath,$ORIGIN", f"-L{libraries}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
@@ -102,7 +115,8 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     jobs = jobs or min(len(sources), os.cpu_count() or 4)
-    with ThreadPoolExecutor(max_workers=jobs) as pool:
+    with ThreadPoolExecutor(max_workers=jobs + 1) as pool:
+        binding = pool.submit(_compile_binding, force)
         results = list(pool.map(lambda s: _compile(s, force, extra or []), sources))
     objects = [obj for obj, _ in results]
     if verbose:
@@ -116,7 +130,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
-    _build_binding(force)
+    _link_binding(binding.result()[0], force)
     return LIBRARY
 
 

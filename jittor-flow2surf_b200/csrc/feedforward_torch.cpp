@@ -24,15 +24,14 @@ using std::optional;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Raise what _lib.check raises for a status.
+// ValueError for what the caller can mend, RuntimeError otherwise, as _lib.check
+// (whose subclass of it a backward, which runs without the interpreter's lock,
+// cannot raise).
 void check(int status) {
     if (status == F2S_OK) return;
     const std::string message = f2s_last_error();
     TORCH_CHECK_VALUE(status != F2S_ERR_INVALID_ARGUMENT && status != F2S_ERR_UNSUPPORTED, message);
-    py::gil_scoped_acquire gil;
-    py::object type = py::module_::import("flow2surf_b200._lib").attr("Flow2SurfError");
-    PyErr_SetObject(type.ptr(), type(status, message).ptr());
-    throw py::error_already_set();
+    TORCH_CHECK(false, "[status ", status, "] ", message);
 }
 
 std::string shape_of(const Tensor& t) {
@@ -232,6 +231,8 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& weight, co
 // Gradients of a step that asks for a second derivative raise once one is taken.
 variable_list once_differentiable(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true);
     auto error = std::make_shared<torch::autograd::DelayedError>(
         "the 8-bit feed-forward operators have no second derivative", (int64_t)grads.size());
     return (*error)(std::move(grads));

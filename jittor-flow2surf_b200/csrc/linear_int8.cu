@@ -96,7 +96,7 @@ int few_launch(const Int8Args& g, cudaStream_t st) {
 template <typename T>
 __global__ void __launch_bounds__(256) linear_int8_any_kernel(const Int8Args g) {
     __shared__ int8_t xa[64][68], wa[64][68];
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
+    const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     int acc[4][4] = {};
     for (int k0 = 0; k0 < g.K; k0 += 64) {
@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(256) linear_int8_any_kernel(const Int8Args g) 
 
 template <typename T>
 int any_launch(const Int8Args& g, cudaStream_t st) {
-    F2S_LIMIT(ceil_div(g.rows, 64) <= 65535, "linear_int8: %d rows of an unaligned pitch", g.rows);
-    linear_int8_any_kernel<T><<<dim3(ceil_div(g.cols, 64), ceil_div(g.rows, 64)), 256, 0, st>>>(g);
+    F2S_LIMIT(ceil_div(g.cols, 64) <= 65535, "linear_int8: %d columns of an unaligned pitch", g.cols);
+    linear_int8_any_kernel<T><<<dim3(ceil_div(g.rows, 64), ceil_div(g.cols, 64)), 256, 0, st>>>(g);
     return check_launch("linear_int8_any_kernel");
 }
 

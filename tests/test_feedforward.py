@@ -8,6 +8,9 @@ equal to the nearest whole numbers of the exact quotient.
 """
 
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -777,6 +780,62 @@ def test_training_captured_and_replayed(cuda):
     graph.replay()
     for a, b in zip(got, step()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_capture_beside_a_live_eager_graph(cuda):
+    """A backward captured while an eager graph of the same leaves is alive cannot
+    be captured (its leaves belong to the eager stream): an error in Python, in a
+    process that lives on."""
+    code = """
+import sys, torch
+sys.path.insert(0, "jittor-flow2surf_b200")
+import flow2surf_b200 as f2s
+x = torch.randn(8, 64, device="cuda", requires_grad=True)
+w = torch.ones(64, device="cuda", requires_grad=True)
+step = lambda: torch.autograd.grad(f2s.swiglu(f2s.add_rms_norm(x, w)[0], checkpoint="int8").sum(), (x, w))
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side):
+    step()
+torch.cuda.current_stream().wait_stream(side)
+alive = f2s.add_rms_norm(x, w)
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        step()
+    print("captured")
+except RuntimeError as error:
+    print("raised")
+print("lives on")
+"""
+    root = Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0 and done.stdout.split()[-2:] == ["lives", "on"], done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused(cuda):
+    x = normal(4, 64, seed=1).to(cuda).requires_grad_()
+    w = normal(64, seed=2).to(cuda).requires_grad_()
+    for out in (f2s.add_rms_norm(x, w)[0], f2s.swiglu(x), f2s.swiglu(x, checkpoint="int8")):
+        gx, = torch.autograd.grad(out.sum(), x, create_graph=True)  # a first one is given
+        with pytest.raises(RuntimeError):  # x is not reached by it
+            torch.autograd.grad(gx.sum(), x, retain_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            gx.sum().backward()
+
+
+@pytest.mark.gpu
+def test_kept_values_that_were_changed_are_refused(cuda):
+    """What a backward reads may not have been written since (its stream, here)."""
+    x, r = (normal(4, 64, seed=s).to(cuda).requires_grad_() for s in (1, 2))
+    w = normal(64, seed=3).to(cuda).requires_grad_()
+    y, stream = f2s.add_rms_norm(x, w, r)
+    with torch.no_grad():
+        stream.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
 
 
 @pytest.mark.gpu
