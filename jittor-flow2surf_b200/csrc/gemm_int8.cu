@@ -39,6 +39,18 @@ __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint
         : "memory");
 }
 
+// Bounded wait on polls, as tc::mbar_wait_poll, that gives up early only for a wait
+// that ran out elsewhere: the error word may hold another kernel's report (a value
+// out of the fp16 range), which is no reason to stop this one.
+__device__ __forceinline__ bool wait_poll(uint64_t* bar, uint32_t parity, int* err) {
+    for (uint32_t i = 0; i < tc::kSpinLimit; ++i) {
+        if (tc::mbar_try_wait_now(bar, parity)) return true;
+        if ((i & 63u) == 63u && *reinterpret_cast<volatile int*>(err) == tc::kTcWaitTimeout) return false;
+    }
+    atomicExch(err, tc::kTcWaitTimeout);
+    return false;
+}
+
 // ---- clusters ----
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -131,7 +143,7 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     if (warp == 0) {
         if (lane == 0) {
             for (int i = ahead; i < blocks; ++i) {
-                if (i >= S && !tc::mbar_wait_poll(&empty[i % S], ((uint32_t)(i / S) & 1u) ^ 1u, g.err)) {
+                if (i >= S && !wait_poll(&empty[i % S], ((uint32_t)(i / S) & 1u) ^ 1u, g.err)) {
                     // let the copies already issued land before the CTA exits:
                     // each stage's last one
                     for (int j = i - S; j < i; ++j) tc::mbar_drain(&full[j % S], (uint32_t)(j / S) & 1u);
@@ -145,7 +157,7 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         if (lane == 0) {
             for (int kb = kb0; kb < kb1; ++kb) {
                 const int i = kb - kb0, s = i % S;
-                if (!tc::mbar_wait_poll(&full[s], (uint32_t)(i / S) & 1u, g.err)) break;
+                if (!wait_poll(&full[s], (uint32_t)(i / S) & 1u, g.err)) break;
                 tc::tc_fence_after();
                 const uint32_t st = tc::smem_u32(smem + (size_t)s * kStage);
                 const uint64_t a = tc::sw128_desc(st), b = tc::sw128_desc(st + kA);
@@ -160,81 +172,83 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
         }
         __syncwarp();
     }
-    if (split > 1) cluster_wait();
-    bool ok = true;
+    // The accumulators come into registers and tensor memory is freed before this
+    // CTA waits for the others of its cluster: one that held it meanwhile, while
+    // another one could not get its own beside a kernel that waits for this
+    // CTA's, would wait forever.
     const int channel = (warp & 3) * 32 + lane;  // a warp reads its TMEM lane quarter
     const int n = n0 + channel;
-    constexpr int kStep = BN < 32 ? 16 : 32;
-    auto store = [&](int m, int acc, float ws, float b) {
-        static_cast<T*>(g.y)[m * g.ldy + n] = from_f32<T>(fmaf((float)acc * __ldg(g.xs + m), ws, b));
-    };
+    bool ok = true;
+    uint32_t v[BN];
     float ws = 0.0f, b = 0.0f;
     if (warp >= 2) {
         if (n < g.cols) {
             ws = __ldg(g.ws + n);
             b = bias_at<T>(g.bias, n);
         }
-        ok = __all_sync(0xffffffffu, tc::mbar_wait_poll(done, 0, g.err));
+        ok = __all_sync(0xffffffffu, wait_poll(done, 0, g.err));
         tc::tc_fence_after();
-        // four tokens at a time go to the CTAs of the cluster in turn, which
-        // finish them
-        const uint32_t mine = tc::smem_u32(partial + rank * 128 + channel);
+        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        if constexpr (BN == 16) {
+            tc::tmem_ld16_issue(from, v);
+            tc::tmem_ld16_wait(v);
+        } else {
 #pragma unroll
-        for (int j0 = 0; j0 < BN; j0 += kStep) {
-            uint32_t v[kStep];
-            const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + j0;
-            if constexpr (kStep == 32) {
-                tc::tmem_ld32_issue(from, v);
-                tc::tmem_ld32_wait(v);
-            } else {
-                tc::tmem_ld16_issue(from, v);
-                tc::tmem_ld16_wait(v);
-            }
-            if (!ok) continue;
-            if (split == 1) {
-                if (n < g.cols) {
-#pragma unroll
-                    for (int j = 0; j < kStep; ++j)
-                        if (m0 + j0 + j < g.rows) store(m0 + j0 + j, (int)v[j], ws, b);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < kStep; j += 4) {
-                    // split is a power of two
-                    const uint32_t four = (uint32_t)(j0 + j) / 4, to = four & (split - 1);
-                    store_cluster(map_rank(mine + (four & ~(uint32_t)(split - 1)) * 2048u, to), v[j], v[j + 1],
-                                  v[j + 2], v[j + 3]);
-                }
+            for (int j = 0; j < BN; j += 32) {
+                uint32_t (&part)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[j]);
+                tc::tmem_ld32_issue(from + j, part);
+                tc::tmem_ld32_wait(part);
             }
         }
+        tc::tc_fence_before();
     }
-    if (split > 1) {
-        cluster_arrive();
-        cluster_wait();
-        if (warp >= 2 && ok && n < g.cols) {
-            for (int four = rank; four < BN / 4; four += split) {
-                const int m = m0 + four * 4;
-                if (m >= g.rows) break;
-                const int4* from = partial + (four - rank) * 128 + channel;
-                int4 acc = from[0];
-                for (int r = 1; r < split; ++r) {
-                    const int4 more = from[r * 128];
-                    acc.x += more.x;
-                    acc.y += more.y;
-                    acc.z += more.z;
-                    acc.w += more.w;
-                }
-                store(m, acc.x, ws, b);
-                if (m + 1 < g.rows) store(m + 1, acc.y, ws, b);
-                if (m + 2 < g.rows) store(m + 2, acc.z, ws, b);
-                if (m + 3 < g.rows) store(m + 3, acc.w, ws, b);
-            }
-        }
-    }
-    tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     if (warp == 1) tc::tmem_dealloc(tmem, kCols);
+
+    auto store = [&](int m, int acc) {
+        static_cast<T*>(g.y)[m * g.ldy + n] = from_f32<T>(fmaf((float)acc * __ldg(g.xs + m), ws, b));
+    };
+    if (split == 1) {
+        if (warp >= 2 && ok && n < g.cols) {
+#pragma unroll
+            for (int j = 0; j < BN; ++j)
+                if (m0 + j < g.rows) store(m0 + j, (int)v[j]);
+        }
+        return;
+    }
+    cluster_wait();
+    if (warp >= 2 && ok) {
+        // four tokens at a time go to the CTAs of the cluster in turn, which
+        // finish them (split is a power of two)
+        const uint32_t mine = tc::smem_u32(partial + rank * 128 + channel);
+#pragma unroll
+        for (int j = 0; j < BN; j += 4) {
+            const uint32_t four = (uint32_t)j / 4, to = four & (split - 1);
+            store_cluster(map_rank(mine + (four & ~(uint32_t)(split - 1)) * 2048u, to), v[j], v[j + 1], v[j + 2],
+                          v[j + 3]);
+        }
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (warp < 2 || !ok || n >= g.cols) return;
+    for (int four = rank; four < BN / 4; four += split) {
+        const int m = m0 + four * 4;
+        if (m >= g.rows) break;
+        const int4* from = partial + (four - rank) * 128 + channel;
+        int4 acc = from[0];
+        for (int r = 1; r < split; ++r) {
+            const int4 more = from[r * 128];
+            acc.x += more.x;
+            acc.y += more.y;
+            acc.z += more.z;
+            acc.w += more.w;
+        }
+        store(m, acc.x);
+        if (m + 1 < g.rows) store(m + 1, acc.y);
+        if (m + 2 < g.rows) store(m + 2, acc.z);
+        if (m + 3 < g.rows) store(m + 3, acc.w);
+    }
 }
 
 int operand_map(CUtensorMap* map, const int8_t* p, int64_t ld, int nrows, int K, int box_rows) {
@@ -437,7 +451,7 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                 int m0, n0;
                 walk.at(g, m0, n0);
                 for (int kb = 0; kb < g.k_blocks; ++kb) {
-                    if (!tc::mbar_wait_poll(&empty[stage], phase ^ 1u, g.err)) {
+                    if (!wait_poll(&empty[stage], phase ^ 1u, g.err)) {
                         ok = false;
                         break;
                     }
@@ -472,11 +486,11 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             bool ok = true;
             for (int t = pair; ok && t < tiles; t += pairs, ++iter) {
                 const int buf = iter & 1;
-                if (!tc::mbar_wait_poll(&tempty[buf], ((uint32_t)(iter >> 1) & 1u) ^ 1u, g.err)) break;
+                if (!wait_poll(&tempty[buf], ((uint32_t)(iter >> 1) & 1u) ^ 1u, g.err)) break;
                 tc::tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)(buf * 256);
                 for (int kb = 0; kb < g.k_blocks; ++kb) {
-                    if (!tc::mbar_wait_poll(&full[stage], phase, g.err)) {
+                    if (!wait_poll(&full[stage], phase, g.err)) {
                         ok = false;
                         break;
                     }
@@ -536,7 +550,7 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             __syncwarp();
             walk.next(g, pairs);
             fetch();
-            const bool ok = tc::mbar_wait_poll(&tfull[buf], (uint32_t)(iter >> 1) & 1u, g.err);
+            const bool ok = wait_poll(&tfull[buf], (uint32_t)(iter >> 1) & 1u, g.err);
             // a warp that gave up stops with its lanes together
             if (!__all_sync(0xffffffffu, ok)) break;
             tc::tc_fence_after();

@@ -548,6 +548,25 @@ def test_linear_int8_large(cuda, rows, cols, K):
 
 
 @pytest.mark.gpu
+def test_linear_int8_forms_at_once(cuda):
+    """Products of every form on their own streams, 20 of each in flight."""
+    shapes = [(2, 512, 1024), (24, 1024, 4096), (60, 300, 2048), (3000, 1024, 1024), (2000, 192, 700)]
+    operands = [(eighths(r, K, i, cuda), eighths(c, K, i + 10, cuda)) for i, (r, c, K) in enumerate(shapes)]
+    want = [f2s.linear_int8(x, w) for x, w in operands]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in shapes]
+    got = [[] for _ in shapes]
+    for _ in range(20):
+        for i, (x, w) in enumerate(operands):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(f2s.linear_int8(x, w))
+    torch.cuda.synchronize()
+    _lib.check_device_error()
+    for w, ys in zip(want, got):
+        assert all(torch.equal(y, w) for y in ys)
+
+
+@pytest.mark.gpu
 def test_linear_int8_scales_that_are_not_finite(cuda):
     x, w = eighths(40, 64, 1, cuda), eighths(50, 64, 2, cuda)
     want = f2s.linear_int8(x, w, dtype=torch.float32)
