@@ -89,95 +89,93 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
     }
 }
 
-// The E channels of a row that thread `t` of TPR holds. kWide: 16-byte
-// vectors (the row's start 16-byte aligned, C a multiple of the vector),
-// vector i of the thread at (i TPR + t); otherwise single values, value i at
-// i TPR + t. Channels past C read as 0 and are not written.
-template <typename T, int E, int TPR, bool kWide>
+// How the threads of a row access it: single values, pairs of a 16-bit type (rows
+// that start on 4 bytes, C even), or 16-byte vectors (rows that start on 16 bytes, C
+// a multiple of the vector).
+enum Mode { kSingle, kPair, kWide };
+
+// The E channels of a row that thread `t` of TPR holds: access i of the thread at
+// (i TPR + t), so that a warp's are adjacent.
+template <typename T, int E, int TPR, Mode kMode>
 struct Slice {
-    static constexpr int V = kWide ? kVec<T> : 1;
-    static_assert(E % V == 0, "whole vectors");
+    static constexpr int V = kMode == kWide ? kVec<T> : kMode == kPair ? 2 : 1;
+    static_assert(E % 8 == 0 && (kMode != kPair || sizeof(T) == 2), "whole chunks; pairs of a 16-bit type");
 
-    __device__ static __forceinline__ int channel(int i, int t) {
-        return ((i / V) * TPR + t) * V + i % V;
-    }
-
-    __device__ static __forceinline__ void load(const T* row, int C, int t, float (&v)[E]) {
-#pragma unroll
-        for (int i = 0; i < E; i += V) {
-            const int c = channel(i, t);
-            if constexpr (kWide) {
-                const uint4 u = c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
-                unpack16<T>(u, &v[i]);
-            } else {
-                v[i] = c < C ? to_f32<T>(row[c]) : 0.0f;
-            }
-        }
-    }
-
-    __device__ static __forceinline__ void store(T* row, int C, int t, const float (&v)[E]) {
-#pragma unroll
-        for (int i = 0; i < E; i += V) {
-            const int c = channel(i, t);
-            if (c >= C) continue;
-            if constexpr (kWide) *reinterpret_cast<uint4*>(row + c) = pack16<T>(&v[i]);
-            else row[c] = from_f32<T>(v[i]);
-        }
-    }
+    __device__ static __forceinline__ int channel(int i, int t) { return ((i / V) * TPR + t) * V + i % V; }
 };
 
-// A thread's E channels as they are stored: packed pairs of a 16-bit type read
-// in vectors (half the registers of fp32 values), fp32 otherwise. Used in
-// chunks of 8.
-template <typename T, int E, bool kWide>
+// A thread's E channels as they are stored: packed pairs of a 16-bit type that is
+// not read value by value (half the registers of fp32 values), fp32 otherwise. Used
+// in chunks of 8. Channels past C are 0 and not written.
+template <typename T, int E, Mode kMode>
 struct Held {
-    static constexpr bool kPacked = kWide && sizeof(T) == 2;
-    static_assert(E % 8 == 0, "whole chunks");
-    uint4 u[kPacked ? E / 8 : 1];
+    static constexpr bool kPacked = kMode != kSingle && sizeof(T) == 2;
+    uint32_t w[kPacked ? E / 2 : 1];
     float f[kPacked ? 1 : E];
 
     __device__ __forceinline__ void get(int i, float (&v)[8]) const {
-        if constexpr (kPacked) {
-            unpack16<T>(u[i / 8], v);
-        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = f[i + j];
+        for (int j = 0; j < 8; j += 2) {
+            if constexpr (kPacked) {
+                const float2 two = unpack2(w[(i + j) / 2], T());
+                v[j] = two.x;
+                v[j + 1] = two.y;
+            } else {
+                v[j] = f[i + j];
+                v[j + 1] = f[i + j + 1];
+            }
         }
     }
     // Values rounded to T.
     __device__ __forceinline__ void set(int i, const float (&v)[8]) {
-        if constexpr (kPacked) {
-            u[i / 8] = pack16<T>(v);
-        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[i + j] = to_f32<T>(from_f32<T>(v[j]));
+        for (int j = 0; j < 8; j += 2) {
+            if constexpr (kPacked) {
+                w[(i + j) / 2] = pack2(v[j], v[j + 1], T());
+            } else {
+                f[i + j] = to_f32<T>(from_f32<T>(v[j]));
+                f[i + j + 1] = to_f32<T>(from_f32<T>(v[j + 1]));
+            }
         }
     }
 };
 
-template <typename S, typename T, int E, bool kWide>
-__device__ __forceinline__ void load_held(const T* row, int C, int t, Held<T, E, kWide>& h) {
-    if constexpr (Held<T, E, kWide>::kPacked) {
+template <int TPR, typename T, int E, Mode kMode>
+__device__ __forceinline__ void load_held(const T* row, int C, int t, Held<T, E, kMode>& h) {
+    using S = Slice<T, E, TPR, kMode>;
 #pragma unroll
-        for (int i = 0; i < E; i += 8) {
-            const int c = S::channel(i, t);
-            h.u[i / 8] = c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < E; i += S::V) {
+        const int c = S::channel(i, t);
+        if constexpr (kMode == kSingle) {
+            h.f[i] = c < C ? to_f32<T>(row[c]) : 0.0f;
+        } else if constexpr (kMode == kPair) {
+            h.w[i / 2] = c < C ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+        } else {
+            const uint4 u = c < C ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+            if constexpr (sizeof(T) == 2) {
+                h.w[i / 2] = u.x;
+                h.w[i / 2 + 1] = u.y;
+                h.w[i / 2 + 2] = u.z;
+                h.w[i / 2 + 3] = u.w;
+            } else {
+                unpack16<T>(u, &h.f[i]);
+            }
         }
-    } else {
-        S::load(row, C, t, h.f);
     }
 }
 
-template <typename S, typename T, int E, bool kWide>
-__device__ __forceinline__ void store_held(T* row, int C, int t, const Held<T, E, kWide>& h) {
-    if constexpr (Held<T, E, kWide>::kPacked) {
+template <int TPR, typename T, int E, Mode kMode>
+__device__ __forceinline__ void store_held(T* row, int C, int t, const Held<T, E, kMode>& h) {
+    using S = Slice<T, E, TPR, kMode>;
 #pragma unroll
-        for (int i = 0; i < E; i += 8) {
-            const int c = S::channel(i, t);
-            if (c < C) *reinterpret_cast<uint4*>(row + c) = h.u[i / 8];
-        }
-    } else {
-        S::store(row, C, t, h.f);
+    for (int i = 0; i < E; i += S::V) {
+        const int c = S::channel(i, t);
+        if (c >= C) continue;
+        if constexpr (kMode == kSingle) row[c] = from_f32<T>(h.f[i]);
+        else if constexpr (kMode == kPair) *reinterpret_cast<uint32_t*>(row + c) = h.w[i / 2];
+        else if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint4*>(row + c) = make_uint4(h.w[i / 2], h.w[i / 2 + 1], h.w[i / 2 + 2], h.w[i / 2 + 3]);
+        else *reinterpret_cast<uint4*>(row + c) = pack16<T>(&h.f[i]);
     }
 }
 
@@ -392,22 +390,28 @@ __device__ __forceinline__ void round8(float (&v)[8], const Rounding<M>& r, uint
     }
 }
 
-// Chunk i of a thread's channels, v, to 8 bits in `row` (of a pitch that keeps
-// vectors aligned where kWide). at(j): value j of the chunk in m's type, scaled.
-template <bool kShort, typename S, bool kWide, typename M, typename F>
+// Chunk i of a thread's channels, v, to 8 bits in `row` (of a start and pitch that
+// keep pairs and vectors aligned). at(j): value j of the chunk in m's type, scaled.
+template <bool kShort, typename S, Mode kMode, typename M, typename F>
 __device__ __forceinline__ void store8_chunk(int8_t* row, int C, int t, int i, float (&v)[8], const Rounding<M>& r,
                                              F at) {
     uint32_t q[8];
     round8<kShort>(v, r, q, at);
     const int c = S::channel(i, t);
-    if constexpr (kWide && S::V == 8) {
+    if constexpr (kMode == kWide && S::V == 8) {
         if (c < C)
             *reinterpret_cast<uint2*>(row + c) =
                 make_uint2(pack_bytes(q[0], q[1], q[2], q[3]), pack_bytes(q[4], q[5], q[6], q[7]));
-    } else if constexpr (kWide) {
+    } else if constexpr (kMode == kWide) {
         const int c4 = S::channel(i + 4, t);
         if (c < C) *reinterpret_cast<uint32_t*>(row + c) = pack_bytes(q[0], q[1], q[2], q[3]);
         if (c4 < C) *reinterpret_cast<uint32_t*>(row + c4) = pack_bytes(q[4], q[5], q[6], q[7]);
+    } else if constexpr (kMode == kPair) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const int c2 = S::channel(i + j, t);
+            if (c2 < C) *reinterpret_cast<uint16_t*>(row + c2) = (uint16_t)__byte_perm(q[j], q[j + 1], 0x0040);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -425,6 +429,11 @@ __device__ __forceinline__ void widen8(uint32_t w, float* v) {
     v[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - 8388736.0f;
 }
 
+// Reciprocal root of a row's mean square from its sum.
+__device__ __forceinline__ float reciprocal_rms(float sum, int C, float eps) {
+    return __frsqrt_rn(sum / (float)C + eps);
+}
+
 // ---- dispatch --------------------------------------------------------------
 // What a kernel's registers hold per channel decides how many channels (of
 // `size` bytes) a thread of a TPR-thread row takes at most.
@@ -439,7 +448,7 @@ constexpr int most_channels(Kind kind, int size, int tpr) {
 constexpr int kThreads[] = {8, 32, 128, 256, 512, 1024};
 
 // Single values of a 16-bit type are held in fp32.
-constexpr int held_size(int size, bool wide) { return wide ? size : 4; }
+constexpr int held_size(int size, Mode mode) { return mode == kSingle ? 4 : size; }
 
 // (TPR, E) for a row of C channels: the fewest threads that hold it, since each
 // thread's share of the reduction and of the row's constants costs as much as
@@ -451,16 +460,18 @@ struct Shape {
     int tpr, e;
 };
 
-inline Shape pick_shape(Kind kind, int size, int64_t nrows, int C, bool wide) {
+inline Shape pick_shape(Kind kind, int size, int64_t nrows, int C, Mode mode) {
+    size = held_size(size, mode);
+    const bool single = mode == kSingle;
     int i = 0;
     while (i < 4 && kThreads[i] * most_channels(kind, size, kThreads[i]) < C) ++i;
     while (i < 4 && C > kThreads[i] * 8 && nrows * kThreads[i] < (int64_t)sm_count() * 512) ++i;
     // single values: 8, 16 or 32; the backward's on 1,024 threads before they spill
     // (8,192 x 4,097: 210 us against 466; the forward 157 against 110)
-    if (kThreads[i] * 32 < C || (!wide && kind == kGrad && i == 4 && C > 512 * 8)) i = 5;
+    if (kThreads[i] * 32 < C || (single && kind == kGrad && i == 4 && C > 512 * 8)) i = 5;
     const int e = ceil_div(ceil_div(C, kThreads[i]), 8) * 8;
-    const bool all = i == 5 && (wide || kind == kForward);
-    return {kThreads[i], all || (!wide && e > 16) ? 32 : e};
+    const bool all = i == 5 && (!single || kind == kForward);
+    return {kThreads[i], all || (single && e > 16) ? 32 : e};
 }
 
 // Blocks of `threads` per SM that E channels held in `size` bytes each leave
@@ -476,45 +487,76 @@ constexpr int block_rows(int tpr) { return tpr <= 32 ? 256 / tpr : 1; }
 template <int kValue>
 using Const = std::integral_constant<int, kValue>;
 
-template <Kind kKind, int kSize, int kTpr, typename F>
-void dispatch_channels(const Shape& s, bool wide, F f) {
-    constexpr int most = kTpr >= 512 ? 32 : most_channels(kKind, kSize, kTpr);
-    constexpr int most_single = kTpr == 1024 || (kTpr == 512 && kKind == kForward) ? 32 : most_channels(kKind, 4, kTpr);
-    if (!wide) {
-        constexpr bool few = kTpr < 1024 || kKind == kGrad;  // a forward of 1,024 threads takes 32
-        if constexpr (few)
-            if (s.e == 8) f(Const<8>(), Const<kTpr>(), std::false_type());
-        if constexpr (few && most_single >= 16)
-            if (s.e == 16) f(Const<16>(), Const<kTpr>(), std::false_type());
-        if constexpr (most_single >= 32)
-            if (s.e == 32) f(Const<32>(), Const<kTpr>(), std::false_type());
-        return;
-    }
-    if constexpr (kTpr < 1024) {
-        if (s.e == 8) f(Const<8>(), Const<kTpr>(), std::true_type());
+template <Mode kValue>
+using ConstMode = std::integral_constant<Mode, kValue>;
+
+template <Kind kKind, int kSize, Mode kMode, int kTpr, typename F>
+void dispatch_channels(const Shape& s, F f) {
+    constexpr bool single = kMode == kSingle;
+    // 512 and 1,024 threads take what is left, but for the backward's single values
+    constexpr int most = kTpr == 1024 || (kTpr == 512 && !(single && kKind == kGrad))
+                             ? 32
+                             : most_channels(kKind, held_size(kSize, kMode), kTpr);
+    if constexpr (kTpr < 1024 || (single && kKind == kGrad)) {
+        if (s.e == 8) f(Const<8>(), Const<kTpr>(), ConstMode<kMode>());
         if constexpr (most >= 16)
-            if (s.e == 16) f(Const<16>(), Const<kTpr>(), std::true_type());
-        if constexpr (most >= 24)
-            if (s.e == 24) f(Const<24>(), Const<kTpr>(), std::true_type());
+            if (s.e == 16) f(Const<16>(), Const<kTpr>(), ConstMode<kMode>());
+        if constexpr (most >= 24 && !single)
+            if (s.e == 24) f(Const<24>(), Const<kTpr>(), ConstMode<kMode>());
     }
     if constexpr (most >= 32)
-        if (s.e == 32) f(Const<32>(), Const<kTpr>(), std::true_type());
+        if (s.e == 32) f(Const<32>(), Const<kTpr>(), ConstMode<kMode>());
 }
 
-// f(E, TPR, wide) for the shape, as integral constants.
-template <Kind kKind, int kSize, typename F>
-void dispatch(const Shape& s, bool wide, F f) {
+template <Kind kKind, int kSize, Mode kMode, typename F>
+void dispatch_threads(const Shape& s, F f) {
     switch (s.tpr) {
-        case 8: dispatch_channels<kKind, kSize, 8>(s, wide, f); break;
-        case 32: dispatch_channels<kKind, kSize, 32>(s, wide, f); break;
-        case 128: dispatch_channels<kKind, kSize, 128>(s, wide, f); break;
-        case 256: dispatch_channels<kKind, kSize, 256>(s, wide, f); break;
-        case 512: dispatch_channels<kKind, kSize, 512>(s, wide, f); break;
-        default: dispatch_channels<kKind, kSize, 1024>(s, wide, f); break;
+        case 8: dispatch_channels<kKind, kSize, kMode, 8>(s, f); break;
+        case 32: dispatch_channels<kKind, kSize, kMode, 32>(s, f); break;
+        case 128: dispatch_channels<kKind, kSize, kMode, 128>(s, f); break;
+        case 256: dispatch_channels<kKind, kSize, kMode, 256>(s, f); break;
+        case 512: dispatch_channels<kKind, kSize, kMode, 512>(s, f); break;
+        default: dispatch_channels<kKind, kSize, kMode, 1024>(s, f); break;
     }
+}
+
+// f(E, TPR, mode) for the shape, as integral constants: T's type decides whether
+// there are pairs, `kSize` (its own, or what a kernel holds) the registers.
+template <Kind kKind, typename T, int kSize = sizeof(T), typename F>
+void dispatch(const Shape& s, Mode mode, F f) {
+    if (mode == kWide) dispatch_threads<kKind, kSize, kWide>(s, f);
+    else if (mode == kSingle) dispatch_threads<kKind, kSize, kSingle>(s, f);
+    if constexpr (sizeof(T) == 2)
+        if (mode == kPair) dispatch_threads<kKind, kSize, kPair>(s, f);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The widest mode that all of a kernel's rows allow.
+struct Layout {
+    int64_t nrows;
+    int vec;
+    bool wide, pairs;
+    Layout(int64_t n, int C, int size)
+        : nrows(n), vec(16 / size), wide(C % (16 / size) == 0), pairs(size == 2 && C % 2 == 0) {}
+    Layout& vector(const void* p) {
+        wide = wide && aligned16(p);
+        pairs = pairs && (reinterpret_cast<uintptr_t>(p) & 3) == 0;
+        return *this;
+    }
+    Layout& rows(const void* p, int64_t pitch) {  // null: none
+        if (!p) return *this;
+        wide = wide && (pitch % vec == 0 || nrows == 1);
+        pairs = pairs && (pitch % 2 == 0 || nrows == 1);
+        return vector(p);
+    }
+    Layout& eight(const void* p, int64_t pitch) {
+        wide = wide && aligned16(p) && (pitch % vec == 0 || nrows == 1);
+        pairs = pairs && (reinterpret_cast<uintptr_t>(p) & 1) == 0 && (pitch % 2 == 0 || nrows == 1);
+        return *this;
+    }
+    Mode mode() const { return wide ? kWide : pairs ? kPair : kSingle; }
+};
 
 // The three element types of these operators (f2s_dtype).
 #define F2S_DTYPE_SWITCH(dtype, ...)                                     \
@@ -527,6 +569,14 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline int check_dtype(const char* what, int dtype) {
     F2S_REQUIRE(dtype == F2S_DTYPE_F32 || dtype == F2S_DTYPE_BF16 || dtype == F2S_DTYPE_F16, "%s: unknown dtype %d",
                 what, dtype);
+    return F2S_OK;
+}
+
+inline int check_norm(const char* what, int dtype, int64_t nrows, int C, float eps) {
+    F2S_TRY(check_dtype(what, dtype));
+    F2S_REQUIRE(nrows >= 0 && C >= 1 && eps >= 0.0f, "%s: bad shape rows=%lld C=%d eps=%g", what,
+                (long long)nrows, C, (double)eps);
+    F2S_LIMIT(C <= kMaxRow, "%s: C=%d, at most %d channels", what, C, kMaxRow);
     return F2S_OK;
 }
 

@@ -9,11 +9,11 @@ namespace {
 
 using namespace rows;
 
-template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, kWide ? sizeof(T) : 4))
+template <typename T, int E, int TPR, Mode kMode>
+__global__ void __launch_bounds__(block_threads(TPR), resident(block_threads(TPR), E, held_size(sizeof(T), kMode)))
 quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t nrows, int width, int8_t* __restrict__ q8,
                      int64_t ldq, float* __restrict__ scale) {
-    using S = Slice<T, E, TPR, kWide>;
+    using S = Slice<T, E, TPR, kMode>;
     __shared__ float shared_m[32];
     const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
     const int64_t row = TPR <= 32 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
@@ -21,8 +21,8 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t nrows, int wi
     const int64_t at = live ? row : 0;
     const int C = live ? width : 0;
     const T* from = x + at * ldx;
-    Held<T, E, kWide> held;
-    load_held<S>(from, C, t, held);
+    Held<T, E, kMode> held;
+    load_held<TPR>(from, C, t, held);
     float m = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; i += 8) {
@@ -36,7 +36,7 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t nrows, int wi
     for (int i = 0; i < E; i += 8) {
         float v[8];
         held.get(i, v);
-        store8_chunk<sizeof(T) == 2, S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
+        store8_chunk<sizeof(T) == 2, S, kMode>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
     }
     if (live && t == 0) scale[row] = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
 }
@@ -88,15 +88,13 @@ dequantize_any_kernel(const int8_t* __restrict__ q8, int64_t ldq, const float* _
 template <typename T>
 int quantize_launch(const void* x, int64_t ldx, int64_t nrows, int C, int8_t* q, int64_t ldq, float* scale,
                     cudaStream_t st) {
-    constexpr int vec = kVec<T>;
-    const bool wide = C % vec == 0 && aligned16(x) && aligned16(q) &&
-                      ((ldx % vec == 0 && ldq % vec == 0) || nrows == 1);
-    const Shape s = pick_shape(kForward, held_size(sizeof(T), wide), nrows, C, wide);
+    const Mode mode = Layout(nrows, C, sizeof(T)).rows(x, ldx).eight(q, ldq).mode();
+    const Shape s = pick_shape(kForward, sizeof(T), nrows, C, mode);
     const int64_t blocks = ceil_div64(nrows, block_rows(s.tpr));
     F2S_LIMIT(blocks <= INT32_MAX, "quantize_rows: %lld rows", (long long)nrows);
     TraceScope trace(kTagRows8, st);
-    dispatch<kForward, sizeof(T)>(s, wide, [&](auto e, auto tpr, auto w) {
-        quantize_rows_kernel<T, e.value, tpr.value, w.value><<<(unsigned)blocks, block_threads(tpr.value), 0, st>>>(
+    dispatch<kForward, T>(s, mode, [&](auto e, auto tpr, auto m) {
+        quantize_rows_kernel<T, e.value, tpr.value, m.value><<<(unsigned)blocks, block_threads(tpr.value), 0, st>>>(
             static_cast<const T*>(x), ldx, nrows, C, q, ldq, scale);
     });
     return check_launch("quantize_rows_kernel");

@@ -184,11 +184,11 @@ swiglu_grad_kernel(const T* __restrict__ projected, int64_t ld, const int8_t* __
 }
 
 // h as 8-bit rows.
-template <typename T, int E, int TPR, bool kWide>
-__global__ void __launch_bounds__(TPR <= 32 ? 256 : TPR, resident(TPR <= 32 ? 256 : TPR, E, 2 * sizeof(T)))
+template <typename T, int E, int TPR, Mode kMode>
+__global__ void __launch_bounds__(block_threads(TPR), resident(block_threads(TPR), E, 2 * sizeof(T)))
 swiglu_int8_kernel(const T* __restrict__ projected, int64_t ld, int64_t nrows, int H, int8_t* __restrict__ q8,
                    int64_t ldq, float* __restrict__ scale) {
-    using S = Slice<T, E, TPR, kWide>;
+    using S = Slice<T, E, TPR, kMode>;
     __shared__ float shared_m[32];
     const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
     const int64_t row = TPR <= 32 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
@@ -196,9 +196,9 @@ swiglu_int8_kernel(const T* __restrict__ projected, int64_t ld, int64_t nrows, i
     const int64_t at = live ? row : 0;
     const int C = live ? H : 0;
     const T* from = projected + at * ld;
-    Held<T, E, kWide> gate, value;
-    load_held<S>(from, C, t, gate);
-    load_held<S>(from + H, C, t, value);
+    Held<T, E, kMode> gate, value;
+    load_held<TPR>(from, C, t, gate);
+    load_held<TPR>(from + H, C, t, value);
     float h[E];
     float m = 0.0f, none = 0.0f;
 #pragma unroll
@@ -220,7 +220,7 @@ swiglu_int8_kernel(const T* __restrict__ projected, int64_t ld, int64_t nrows, i
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = h[i + j];
-        store8_chunk<false, S, kWide>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
+        store8_chunk<false, S, kMode>(q8 + at * ldq, C, t, i, v, rounding, [&](int j) { return v[j]; });
     }
     if (live && t == 0) scale[row] = m < kInf ? m / 127.0f : __int_as_float(0x7fc00000);
 }
@@ -285,15 +285,13 @@ int swiglu_grad_launch(const void* projected, int64_t ld, const int8_t* kept, co
 template <typename T>
 int swiglu_int8_launch(const void* projected, int64_t ld, int64_t nrows, int H, int8_t* q, int64_t ldq, float* scale,
                        cudaStream_t st) {
-    constexpr int vec = kVec<T>;
-    const bool wide = H % vec == 0 && aligned16(projected) && aligned16(q) &&
-                      ((ld % vec == 0 && ldq % vec == 0) || nrows == 1);
-    const Shape s = pick_shape(kForward, 4, nrows, H, wide);  // h is held in fp32
+    const Mode mode = Layout(nrows, H, sizeof(T)).rows(projected, ld).eight(q, ldq).mode();
+    const Shape s = pick_shape(kForward, 4, nrows, H, mode);  // h is held in fp32
     const int64_t blocks = ceil_div64(nrows, block_rows(s.tpr));
     F2S_LIMIT(blocks <= INT32_MAX, "swiglu_int8: %lld rows", (long long)nrows);
     TraceScope trace(kTagSwiGlu, st);
-    dispatch<kForward, 4>(s, wide, [&](auto e, auto tpr, auto w) {
-        swiglu_int8_kernel<T, e.value, tpr.value, w.value><<<(unsigned)blocks, block_threads(tpr.value), 0, st>>>(
+    dispatch<kForward, T, 4>(s, mode, [&](auto e, auto tpr, auto m) {
+        swiglu_int8_kernel<T, e.value, tpr.value, m.value><<<(unsigned)blocks, block_threads(tpr.value), 0, st>>>(
             static_cast<const T*>(projected), ld, nrows, H, q, ldq, scale);
     });
     return check_launch("swiglu_int8_kernel");
