@@ -610,12 +610,13 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     // any pitch: the box's rows one by one, lanes along the row
                     __syncwarp();
                     const T* held = reinterpret_cast<const T*>(box);
-                    for (int r = 0; r < 32 && row0 + r < g.rows; ++r) {
-                        T* to = static_cast<T*>(g.y) + (int64_t)(row0 + r) * g.ldy + col0 + c;
+                    T* to = static_cast<T*>(g.y) + (int64_t)row0 * g.ldy + col0 + c;
+#pragma unroll 8
+                    for (int r = 0; r < 32; ++r, to += g.ldy) {
 #pragma unroll
                         for (int k = lane; k < kBoxCols; k += 32) {
                             const int chunk = k * (int)sizeof(T) / 16, in = k % (16 / (int)sizeof(T));
-                            if (col0 + c + k < g.cols)
+                            if (row0 + r < g.rows && col0 + c + k < g.cols)
                                 to[k] = held[(r * 128 + ((chunk ^ (r & 7)) << 4)) / (int)sizeof(T) + in];
                         }
                     }

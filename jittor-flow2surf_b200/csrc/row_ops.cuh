@@ -6,9 +6,10 @@
 // with shuffles; 128 and up: one row per block), and everything that needs it is
 // computed from there in fp32.
 //
-// Tried and not kept, on a B200: rows of any start by aligned vectors from the
-// boundary before them (8,192 x 4,097 fp16 110 -> 74 us, but 65,536 x 191 29 -> 36,
-// with 8-bit rows 40 -> 53, for the values at a row's ends and the weights).
+// Tried and not kept, on a B200: rows of any start by aligned vectors or pairs from
+// the boundary before them (8,192 x 4,097 fp16 110 -> 74 and 65 us, but 65,536 x 191
+// 29 -> 36 and 33, with 8-bit rows 36 -> 53 and 48: the values at a row's ends and
+// the weights, which start elsewhere, cost narrow rows more than they gain).
 #pragma once
 
 #include <cuda_bf16.h>
