@@ -386,8 +386,8 @@ __device__ __forceinline__ void arrive_pair(uint32_t bar) {
 }
 
 // Eight epilogue warps, two per TMEM lane quarter with every other box of 128
-// bytes of y. (Sixteen, on two accumulators by turns, were slower: 64 us against
-// 58 for 65,536 x 192 -> 1,536, at 96 registers a thread.)
+// bytes of y. (Sixteen, on two accumulators by turns, were no faster: 54 us against
+// 53 for 65,536 x 192 -> 1,536 fp16, 84 against 73 for fp32.)
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -557,29 +557,32 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             const uint32_t acc = tmem + (uint32_t)(buf * 256) + ((uint32_t)(quarter * 32) << 16);
             int held_at = 0;  // this box's columns in ws, bs
             for (int c = half * kBoxCols; c < g.bn; c += 2 * kBoxCols, held_at += kBoxCols) {
-                uint32_t packed[32];  // 128 bytes of y: this lane's row of the box
+                // 32 columns at a time through registers into the box: 128 bytes of y per
+                // lane and row, its 16-byte chunks swizzled
 #pragma unroll
                 for (int p = 0; p < kBoxCols; p += 32) {
                     uint32_t v[32];
                     tc::tmem_ld32_issue(acc + c + p, v);
                     tc::tmem_ld32_wait(v);
+                    if (p == 0) {
+                        // the previous store has read this box
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+                    }
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 w4 = *reinterpret_cast<const float4*>(ws + held_at + p + j);
-                        const float4 b4 = *reinterpret_cast<const float4*>(bs + held_at + p + j);
-                        const float f0 = fmaf((float)(int)v[j] * xs, w4.x, b4.x);
-                        const float f1 = fmaf((float)(int)v[j + 1] * xs, w4.y, b4.y);
-                        const float f2 = fmaf((float)(int)v[j + 2] * xs, w4.z, b4.z);
-                        const float f3 = fmaf((float)(int)v[j + 3] * xs, w4.w, b4.w);
-                        if constexpr (sizeof(T) == 4) {
-                            packed[j] = __float_as_uint(f0);
-                            packed[j + 1] = __float_as_uint(f1);
-                            packed[j + 2] = __float_as_uint(f2);
-                            packed[j + 3] = __float_as_uint(f3);
-                        } else {
-                            packed[(p + j) / 2] = rows::pack2(f0, f1, T());
-                            packed[(p + j) / 2 + 1] = rows::pack2(f2, f3, T());
+                    for (int j = 0; j < 32; j += 16 / (int)sizeof(T)) {
+                        float f[16 / sizeof(T)];
+#pragma unroll
+                        for (int k = 0; k < 16 / (int)sizeof(T); k += 4) {
+                            const float4 w4 = *reinterpret_cast<const float4*>(ws + held_at + p + j + k);
+                            const float4 b4 = *reinterpret_cast<const float4*>(bs + held_at + p + j + k);
+                            f[k] = fmaf((float)(int)v[j + k] * xs, w4.x, b4.x);
+                            f[k + 1] = fmaf((float)(int)v[j + k + 1] * xs, w4.y, b4.y);
+                            f[k + 2] = fmaf((float)(int)v[j + k + 2] * xs, w4.z, b4.z);
+                            f[k + 3] = fmaf((float)(int)v[j + k + 3] * xs, w4.w, b4.w);
                         }
+                        const int q = (p + j) * (int)sizeof(T) / 16;
+                        *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = rows::pack16<T>(f);
                     }
                 }
                 if (c + 2 * kBoxCols >= g.bn) {
@@ -589,13 +592,6 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     if (lane == 0) arrive_pair(to_leader[buf]);
                 }
                 if (col0 + c >= g.cols) continue;  // past the last column
-                // the previous store has read this box
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                __syncwarp();
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                        make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
                 if (g.boxes) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
