@@ -387,7 +387,8 @@ __device__ __forceinline__ void arrive_pair(uint32_t bar) {
 
 // Eight epilogue warps, two per TMEM lane quarter with every other box of 128
 // bytes of y. (Sixteen, on two accumulators by turns, were no faster: 54 us against
-// 53 for 65,536 x 192 -> 1,536 fp16, 84 against 73 for fp32.)
+// 53 for 65,536 x 192 -> 1,536 fp16, 84 against 73 for fp32; two boxes of a warp by
+// turns took 52 and 82.)
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
