@@ -385,10 +385,41 @@ __device__ __forceinline__ void arrive_pair(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// 16 lanes x 64 columns of TMEM: register 4 j + 2 i + k holds lane t / 4 + 8 i of
+// column 8 j + 2 (t % 4) + k, for thread t.
+__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+// Four 8 x 8 matrices of 16-bit values, a thread holding row t / 4, columns 2 (t % 4)
+// and the next of each; lane 8 i + k points at row k of matrix i.
+__device__ __forceinline__ void store_matrices(unsigned char* to, const uint32_t (&r)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(tc::smem_u32(to)), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
+
+// The warp's last store has read its box.
+__device__ __forceinline__ void box_free(int lane) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+}
+
 // Eight epilogue warps, two per TMEM lane quarter with every other box of 128
-// bytes of y. (Sixteen, on two accumulators by turns, were no faster: 54 us against
-// 53 for 65,536 x 192 -> 1,536 fp16, 84 against 73 for fp32; two boxes of a warp by
-// turns took 52 and 82.)
+// bytes of y. Where K is small their shared memory traffic bounds the kernel: a
+// 16-bit y with a whole row in a lane, which takes every scale and bias to every
+// lane, takes 53 us for 65,536 x 192 -> 1,536 against 49 for the split of rows
+// below. A 32-bit y is bound by its writes (75 us, 5.4 TB/s). With a row in a lane
+// sixteen warps, on two accumulators by turns, took 54 (16-bit) and 84 us (32-bit),
+// and two boxes of a warp by turns 52 and 82.
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -543,6 +574,9 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             const int buf = iter & 1;
             const int row0 = m0 + (int)rank * 128 + quarter * 32, col0 = n0;
             const float xs = xs_next;
+            float xs4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) xs4[i] = __shfl_sync(0xffffffffu, xs, (lane >> 2) + 8 * i);
 #pragma unroll
             for (int i = 0; i < kCols / 32; ++i) {
                 ws[lane + 32 * i] = ws_next[i];
@@ -558,32 +592,50 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             const uint32_t acc = tmem + (uint32_t)(buf * 256) + ((uint32_t)(quarter * 32) << 16);
             int held_at = 0;  // this box's columns in ws, bs
             for (int c = half * kBoxCols; c < g.bn; c += 2 * kBoxCols, held_at += kBoxCols) {
-                // 32 columns at a time through registers into the box: 128 bytes of y per
-                // lane and row, its 16-byte chunks swizzled
-#pragma unroll
-                for (int p = 0; p < kBoxCols; p += 32) {
+                // through registers into the box, 128 bytes of y per row, its 16-byte chunks
+                // swizzled
+                if constexpr (sizeof(T) == 4) {
+                    // a lane's row
                     uint32_t v[32];
-                    tc::tmem_ld32_issue(acc + c + p, v);
+                    tc::tmem_ld32_issue(acc + c, v);
                     tc::tmem_ld32_wait(v);
-                    if (p == 0) {
-                        // the previous store has read this box
-                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        __syncwarp();
+                    box_free(lane);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 w4 = *reinterpret_cast<const float4*>(ws + held_at + j);
+                        const float4 b4 = *reinterpret_cast<const float4*>(bs + held_at + j);
+                        *reinterpret_cast<float4*>(box + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) =
+                            make_float4(fmaf((float)(int)v[j] * xs, w4.x, b4.x), fmaf((float)(int)v[j + 1] * xs, w4.y, b4.y),
+                                        fmaf((float)(int)v[j + 2] * xs, w4.z, b4.z), fmaf((float)(int)v[j + 3] * xs, w4.w, b4.w));
+                    }
+                } else {
+                    // columns 8 j + 2 (lane % 4) and the next one of the rows lane / 4 + 8 i: with
+                    // these, a lane reads 32 scales and biases of the box, not 128
+                    float2 w2[8], b2[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        w2[j] = *reinterpret_cast<const float2*>(ws + held_at + 8 * j + 2 * (lane & 3));
+                        b2[j] = *reinterpret_cast<const float2*>(bs + held_at + 8 * j + 2 * (lane & 3));
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; j += 16 / (int)sizeof(T)) {
-                        float f[16 / sizeof(T)];
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t v[32];
+                        tmem_ld16_issue(acc + c + ((uint32_t)(16 * h) << 16), v);
+                        tc::tmem_ld32_wait(v);
+                        if (h == 0) box_free(lane);
 #pragma unroll
-                        for (int k = 0; k < 16 / (int)sizeof(T); k += 4) {
-                            const float4 w4 = *reinterpret_cast<const float4*>(ws + held_at + p + j + k);
-                            const float4 b4 = *reinterpret_cast<const float4*>(bs + held_at + p + j + k);
-                            f[k] = fmaf((float)(int)v[j + k] * xs, w4.x, b4.x);
-                            f[k + 1] = fmaf((float)(int)v[j + k + 1] * xs, w4.y, b4.y);
-                            f[k + 2] = fmaf((float)(int)v[j + k + 2] * xs, w4.z, b4.z);
-                            f[k + 3] = fmaf((float)(int)v[j + k + 3] * xs, w4.w, b4.w);
+                        for (int j = 0; j < 8; j += 2) {
+                            uint32_t y8[4];  // rows 0-7 and 8-15 of columns 8 j .., then of 8 j + 8 ..
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int n = j + k / 2, at = 4 * n + 2 * (k & 1);
+                                const float scale = xs4[2 * h + (k & 1)];
+                                y8[k] = rows::pack2(fmaf((float)(int)v[at] * scale, w2[n].x, b2[n].x),
+                                                    fmaf((float)(int)v[at + 1] * scale, w2[n].y, b2[n].y), T());
+                            }
+                            const int r = 16 * h + (lane & 15);  // the row that this lane points at
+                            store_matrices(box + r * 128 + (((j + (lane >> 4)) ^ (r & 7)) << 4), y8);
                         }
-                        const int q = (p + j) * (int)sizeof(T) / 16;
-                        *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = rows::pack16<T>(f);
                     }
                 }
                 if (c + 2 * kBoxCols >= g.bn) {
