@@ -186,7 +186,8 @@ typedef enum f2s_dtype { F2S_DTYPE_F32 = 0, F2S_DTYPE_BF16 = 1, F2S_DTYPE_F16 = 
  * (ld >= C). Any alignment and pitch is taken; bases and pitches of whole
  * 16-byte vectors (and C a multiple of the vector) are read and written 16
  * bytes at a time. C at most 32768 where a kernel holds a row in registers
- * (F2S_ERR_UNSUPPORTED beyond). All arithmetic is fp32.
+ * (F2S_ERR_UNSUPPORTED beyond). All arithmetic is fp32. Outputs overlap neither
+ * inputs nor one another.
  *
  * 8-bit rows: q (rows, C) int8 of pitch ldq and one fp32 scale per row, standing
  * for scale * q. q is the whole number nearest to 127 v / max|v| (of the exact

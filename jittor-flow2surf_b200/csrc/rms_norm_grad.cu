@@ -37,6 +37,57 @@ constexpr int grad_resident(int tpr, int E, int size, Mode mode) {
     return threads / block_threads(tpr) > 0 ? threads / block_threads(tpr) : 1;
 }
 
+// The block's rows once more, for a block that met a row whose squares leave fp32:
+// by the whole block, value by value, each row's values multiplied by a power of two
+// where they are squared. Apart from the rows' own loop, whose registers it would
+// cost (from within, 170 us became 173 to 245 for 32,768 x 4,096).
+template <typename T>
+__device__ void rows_again(const NormGradArgs& g, int rows_at_once, float* shared_a, float* shared_b) {
+    const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const T* w = static_cast<const T*>(g.weight);
+    float* mine = g.partial ? g.partial + (int64_t)blockIdx.x * g.C : nullptr;
+    auto join = [&](float v, float* shared, bool largest) {
+        v = largest ? lanes_max<32>(v) : lanes_sum<32>(v);
+        __syncthreads();
+        if (lane == 0) shared[warp] = v;
+        __syncthreads();
+        v = lane < threads / 32 ? shared[lane] : 0.0f;
+        return largest ? lanes_max<32>(v) : lanes_sum<32>(v);
+    };
+    if (mine)
+        for (int c = threadIdx.x; c < g.C; c += threads) mine[c] = 0.0f;
+    const int64_t stride = (int64_t)gridDim.x * rows_at_once;
+    for (int64_t first = (int64_t)blockIdx.x * rows_at_once; first < g.nrows; first += stride) {
+        const int64_t last = first + rows_at_once < g.nrows ? first + rows_at_once : g.nrows;
+        for (int64_t row = first; row < last; ++row) {
+            const T* s = static_cast<const T*>(g.s) + row * g.lds;
+            const T* dy = static_cast<const T*>(g.dy) + row * g.lddy;
+            const T* ds = g.ds ? static_cast<const T*>(g.ds) + row * g.ldds : nullptr;
+            T* dx = static_cast<T*>(g.dx) + row * (int64_t)g.C;
+            float m = 0.0f, sum = 0.0f, along = 0.0f;
+            for (int c = threadIdx.x; c < g.C; c += threads) m = max_abs(m, m, to_f32<T>(s[c]));
+            m = join(m, shared_a, true);
+            const float by = square_scale(m * m * (float)g.C, g.eps);  // C m^2 bounds the sum
+            for (int c = threadIdx.x; c < g.C; c += threads) {
+                const float a = to_f32<T>(s[c]) * by;
+                sum = fmaf(a, a, sum);
+                along = fmaf(to_f32<T>(dy[c]) * to_f32<T>(w[c]), a, along);
+            }
+            sum = join(sum, shared_a, false);
+            along = join(along, shared_b, false);
+            const float norm = reciprocal_rms(sum, g.C, g.eps * by * by), rstd = norm * by;
+            const float mean = along * norm / (float)g.C;
+            for (int c = threadIdx.x; c < g.C; c += threads) {
+                const float d = to_f32<T>(dy[c]), n = to_f32<T>(s[c]) * rstd;
+                float grad = rstd * (d * to_f32<T>(w[c]) - n * mean);
+                if (ds) grad += to_f32<T>(ds[c]);
+                dx[c] = from_f32<T>(grad);
+                if (mine) mine[c] = fmaf(d, n, mine[c]);
+            }
+        }
+    }
+}
+
 template <typename T, int E, int TPR, Mode kMode>
 __global__ void __launch_bounds__(block_threads(TPR), grad_resident(TPR, E, held_size(sizeof(T), kMode), kMode))
 add_rms_norm_grad_kernel(const NormGradArgs g) {
@@ -65,6 +116,7 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
     const int64_t stride = (int64_t)gridDim.x * kRows;
     if constexpr (kAhead) fetch(blockIdx.x);
     int parity = 0;
+    bool again = false;
     for (int64_t first = (int64_t)blockIdx.x * kRows; first < g.nrows; first += stride) {
         const int64_t row = first + group;
         const bool live = row < g.nrows;
@@ -75,7 +127,7 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
         dy = dy_next;
         ds = ds_next;
         if constexpr (kAhead) fetch(row + stride);
-        float sum = 0.0f, along = 0.0f;
+        float sum = 0.0f, along = 0.0f;  // s^2, dy w s
 #pragma unroll
         for (int i = 0; i < E; i += 8) {
             float a[8], b[8], c[8];
@@ -104,6 +156,7 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
             along = lanes_sum<kWarps>(shared_b[parity][lane % kWarps]);
             parity ^= 1;
         }
+        again = again || (live && square_scale(sum, g.eps) != 1.0f);
         // 0 past the last row: with eps = 0 its reciprocal would put NaN into dw
         const float rstd = live ? reciprocal_rms(sum, g.C, g.eps) : 0.0f;
         const float mean = along * rstd / (float)g.C;  // mean(u n)
@@ -124,6 +177,13 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
             s.set(i, a);
         }
         store_held<TPR>(static_cast<T*>(g.dx) + at * (int64_t)g.C, C, t, s);
+    }
+    // fp16 has no such rows
+    if constexpr (!std::is_same<T, __half>::value) {
+        if (__syncthreads_or(again)) {
+            rows_again<T>(g, kRows, shared_a[0], shared_b[0]);
+            return;
+        }
     }
     if (!g.partial) return;
     float* mine = g.partial + (int64_t)blockIdx.x * g.C;

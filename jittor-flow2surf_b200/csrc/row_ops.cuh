@@ -99,6 +99,7 @@ enum Mode { kSingle, kPair, kWide };
 // (i TPR + t), so that a warp's are adjacent.
 template <typename T, int E, int TPR, Mode kMode>
 struct Slice {
+    static constexpr int kEach = E;
     static constexpr int V = kMode == kWide ? kVec<T> : kMode == kPair ? 2 : 1;
     static_assert(E % 8 == 0 && (kMode != kPair || sizeof(T) == 2), "whole chunks; pairs of a 16-bit type");
 
@@ -428,6 +429,21 @@ __device__ __forceinline__ void widen8(uint32_t w, float* v) {
     v[1] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - 8388736.0f;
     v[2] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - 8388736.0f;
     v[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - 8388736.0f;
+}
+
+// What a row's values are multiplied by before their squares are summed again,
+// where the sum of the squares themselves is outside of what fp32 holds well (rows
+// of magnitudes above 1e18, or below 1e-14 with an eps that does not hide them).
+// fp16 has no values of the first kind and its squares are never below 2^-48.
+__device__ __forceinline__ float square_scale(float sum, float eps) {
+    return sum > 0x1p120f ? 0x1p-80f : sum < 0x1p-90f && eps < 0x1p-90f ? 0x1p100f : 1.0f;
+}
+// Whether to do that: true for all of the threads that share a row or a warp.
+template <typename T, int TPR>
+__device__ __forceinline__ bool sums_again(float scale) {
+    if constexpr (std::is_same<T, __half>::value) return false;
+    else if constexpr (TPR < 32) return __any_sync(0xffffffffu, scale != 1.0f);
+    else return scale != 1.0f;
 }
 
 // Reciprocal root of a row's mean square from its sum.

@@ -337,6 +337,38 @@ def test_norm_of_rows_without_a_norm(cuda, dtype):
     assert torch.isnan(y[5]).all() and torch.isfinite(y[keep]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [24, 192, 191, 1530, 4096, 16391])
+def test_norm_of_rows_whose_squares_leave_fp32(cuda, width, dtype):
+    """Rows of 1e25 and 1e-25 among ordinary ones, with eps = 0. Their values are
+    multiplied by a power of two before they are squared, which rounds nothing,
+    so the bounds are those of the ordinary rows."""
+    x = normal(9, width, dtype=dtype, seed=width)
+    x[[1, 8]] *= 1e25
+    x[[2, 5]] *= 1e-25
+    x = x.to(cuda).requires_grad_()
+    w = normal(width, dtype=dtype, seed=1).to(cuda).requires_grad_()
+    dy = normal(9, width, dtype=dtype, seed=2).to(cuda)
+    _, s, w64, rstd = norm64(x.detach(), w.detach(), None, 0.0)
+    y, _ = f2s.add_rms_norm(x, w, eps=0.0)
+    y64 = s * rstd * w64
+    close(y.detach(), y64, y64.abs() * (half_step(dtype) + NORM * U) * 1.001 + smallest(dtype))
+    with torch.no_grad():
+        eight, _ = f2s.add_rms_norm_int8(x, w, eps=0.0)
+    p = s * w64
+    assert torch.equal(eight.values, nearest_whole(p, row_max(p)))
+    scale = (row_max(p) * rstd / 127)[:, 0]
+    close(eight.scale, scale, scale * (NORM + 2) * U)
+    got_dx, got_dw = torch.autograd.grad(y, (x, w), dy)
+    dx, dw, (rstd, u, n) = norm_grad64(x.detach(), w.detach(), dy, None, 0.0)
+    mean = (u * n).abs().mean(-1, keepdim=True)
+    bound = half_step(dtype) * dx.abs() + U * (rstd * ((NORM + 4) * u.abs() + (DEPTH + 3 * NORM + 6) * n.abs() * mean))
+    close(got_dx, dx, bound * 1.001 + smallest(dtype))
+    terms = (dy.double() * n).abs().sum(0)
+    close(got_dw, dw, half_step(dtype) * dw.abs() + U * (9 + NORM + 1) * terms + smallest(dtype))
+
+
 # ---- 8-bit rows ----
 
 
