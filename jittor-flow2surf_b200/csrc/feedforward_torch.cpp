@@ -136,6 +136,8 @@ void check_eight(const char* name, const Tensor& values, const Tensor& scale) {
     TORCH_CHECK_VALUE(scale.sizes() == values.sizes().slice(0, values.dim() - 1), name, ": scales ", shape_of(scale),
                       " do not match values ", shape_of(values));
     check_device(values, {&scale});
+    TORCH_CHECK_VALUE(!needs_grad({&scale}), name,
+                      ": 8-bit rows have no gradient, their scales neither; call under torch.no_grad()");
 }
 
 std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {

@@ -46,7 +46,8 @@ class Int8Rows(NamedTuple):
     """Rows in 8 bits: `values` (..., channels) int8 and `scale` (...) float32,
     standing for values * scale[..., None]. The library's rows start on
     multiples of 16 bytes, which the tensor-core product needs; `values` is
-    then a view of a wider buffer where channels is not a multiple of 16."""
+    then a view of a wider buffer where channels is not a multiple of 16. Scales
+    that want a gradient are refused, since none would come."""
 
     values: torch.Tensor
     scale: torch.Tensor

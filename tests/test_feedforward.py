@@ -502,6 +502,18 @@ def test_eight_bit_calls_refuse_gradients(cuda):
         f2s.quantize_rows(torch.zeros(1, 32769, device=cuda))
 
 
+@pytest.mark.gpu
+def test_scales_that_want_a_gradient_are_refused(cuda):
+    eight = f2s.quantize_rows(normal(4, 16, seed=1).to(cuda))
+    learnt = Int8Rows(eight.values, eight.scale.clone().requires_grad_())
+    for call in (lambda: learnt.dequantize(), lambda: f2s.linear_int8(learnt, eight),
+                 lambda: f2s.linear_int8(eight, learnt)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 # ---- the product ----
 
 
