@@ -276,10 +276,10 @@ __device__ __forceinline__ float half_side(float v, float m, float c) {
     const float p = __fmul_rn(254.0f, v), q = __fmul_rn(c, m);
     return __fadd_rn(__fsub_rn(p, q), __fsub_rn(__fmaf_rn(254.0f, v, -p), __fmaf_rn(c, m, -q)));
 }
-// The same of a product v = s w of fp32 values and a 64-bit m: v has 48 bits and
-// 254 v 56, of which 53 are kept.
-__device__ __forceinline__ float half_side(double v, double m, float c) {
-    return (float)(254.0 * v - (double)c * m);
+// The same in 64 bits, of products v and m of two fp32 values (48 bits each).
+__device__ __forceinline__ double half_side(double v, double m, float c) {
+    const double p = __dmul_rn(254.0, v), q = __dmul_rn((double)c, m);
+    return __dadd_rn(__dsub_rn(p, q), __dsub_rn(__fma_rn(254.0, v, -p), __fma_rn((double)c, m, -q)));
 }
 
 __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -380,9 +380,9 @@ __device__ __forceinline__ void round8(float (&v)[8], const Rounding<M>& r, uint
             if (fabsf(d) > kBorder) {
                 // the half between `below` and the next whole number
                 const float below = d > 0.0f ? whole : whole - 1.0f;
-                const float side = half_side(at(j), r.m, 2.0f * below + 1.0f);
+                const auto side = half_side(at(j), r.m, 2.0f * below + 1.0f);
                 const int k = (int)below;
-                q[j] = (uint32_t)(side > 0.0f || (side == 0.0f && (k & 1)) ? k + 1 : k);
+                q[j] = (uint32_t)(side > 0 || (side == 0 && (k & 1)) ? k + 1 : k);
             }
         }
     }
