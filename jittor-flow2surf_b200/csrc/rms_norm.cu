@@ -54,11 +54,68 @@ __device__ __noinline__ float scaled_sum(const T* s, int C, int t, float up) {
     return sum;
 }
 
-// k8: 8-bit rows. The products s w of a 16-bit type are exact in fp32; those of
-// fp32 are taken in 64 bits for the maximum and at rounding borders.
+// The row, so that what follows from it is computed anew.
+__device__ __forceinline__ int64_t opaque(int64_t row) {
+    asm volatile("" : "+l"(row));
+    return row;
+}
+
+// A row whose largest product s w lies outside of [1e-30, 1e30], to 8 bits: products
+// beyond 3.4e38 are infinite in fp32 and those below 1.2e-38 lose bits, so they are
+// taken in 64 bits, which hold every one of them exactly. Almost no row needs it: it
+// reads the row and the weight again, value by value, in a call of its own that is given
+// the row's number alone, so that it takes no registers from the others.
+template <typename T, int E, int TPR, Mode kMode>
+__device__ __noinline__ void products_to_8_bits(const NormArgs& g, int64_t row, float rstd) {
+    using S = Slice<T, E, TPR, kMode>;
+    const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
+    const bool live = row < g.nrows;
+    const int C = live ? g.C : 0;
+    if (!live) row = 0;
+    // the stream: x, or this thread's own channels of it
+    const T* s = g.residual ? static_cast<const T*>(g.stream) + row * (int64_t)g.C
+                            : static_cast<const T*>(g.x) + row * g.ldx;
+    const T* w = static_cast<const T*>(g.weight);
+    int8_t* q = g.q + row * g.ldq;
+    __shared__ unsigned long long shared_m[32];
+    float none = 0.0f;
+    unsigned long long bits = 0;
+#pragma unroll 1
+    for (int i = 0; i < S::kEach; ++i) {
+        const int c = S::channel(i, t);
+        if (c >= C) break;
+        const double p = fabs((double)to_f32<T>(s[c]) * (double)to_f32<T>(w[c]));
+        const unsigned long long b = (unsigned long long)__double_as_longlong(p);
+        bits = b > bits ? b : bits;
+    }
+    row_sum_max<TPR, false, true>(none, bits, &none, shared_m);
+    const double m = __longlong_as_double((long long)bits);
+    const bool finite = m < (double)kInf;
+#pragma unroll 1
+    for (int i = 0; i < S::kEach; ++i) {
+        const int c = S::channel(i, t);
+        if (c >= C) break;
+        const double p = (double)to_f32<T>(s[c]) * (double)to_f32<T>(w[c]);
+        q[c] = (int8_t)(finite && m > 0.0 ? nearest_whole(p, m) : 0);
+    }
+    if (live && t == 0) g.scale[row] = finite ? (float)(m / 127.0 * (double)rstd) : __int_as_float(0x7fc00000);
+}
+
+// 8 single bf16 values with 8-bit rows stay at 48 registers for a fifth 256-thread
+// block per SM: 65,536 x 191 36 us against 41.
 template <typename T, int E, int TPR, Mode kMode, bool k8>
-__global__ void __launch_bounds__(block_threads(TPR), resident(block_threads(TPR), E, 2 * held_size(sizeof(T), kMode)))
-add_rms_norm_kernel(const NormArgs g) {
+constexpr int norm_resident() {
+    constexpr int threads = block_threads(TPR);
+    if (k8 && kMode == kSingle && E == 8 && std::is_same<T, __nv_bfloat16>::value && threads <= 256) return 1280 / threads;
+    return resident(threads, E, 2 * held_size(sizeof(T), kMode));
+}
+
+// k8: 8-bit rows. The products s w of a 16-bit type are exact in fp32 where they stay
+// in its range; those of fp32 are taken in 64 bits for the maximum and at rounding
+// borders.
+template <typename T, int E, int TPR, Mode kMode, bool k8>
+__global__ void __launch_bounds__(block_threads(TPR), norm_resident<T, E, TPR, kMode, k8>())
+add_rms_norm_kernel(const __grid_constant__ NormArgs g) {
     using S = Slice<T, E, TPR, kMode>;
     constexpr bool kExact64 = k8 && sizeof(T) == 4;
     using M = typename std::conditional<kExact64, unsigned long long, float>::type;
@@ -95,6 +152,8 @@ add_rms_norm_kernel(const NormArgs g) {
     }
     float sum = 0.0f;
     M m = 0;
+    uint32_t seen = 0;
+    if constexpr (k8 && std::is_same<T, __nv_bfloat16>::value) seen = s.magnitudes();
 #pragma unroll
     for (int i = 0; i < E; i += 8) {
         float a[8], b[8];
@@ -147,7 +206,7 @@ add_rms_norm_kernel(const NormArgs g) {
                 // `from` holds the stream: x, or this thread's own channels of it
                 store8_chunk<false, S, kMode>(g.q + at * g.ldq, C, t, i, a, rounding, [&](int j) {
                     const int c = S::channel(i + j, t);
-                    return c < C ? (double)from[c] * (double)weight[c] * (double)rounding.scale : 0.0;
+                    return c < C ? (double)from[c] * (double)weight[c] : 0.0;
                 });
             } else {
                 // products of bf16 have 16 bits, of fp16 22
@@ -158,6 +217,17 @@ add_rms_norm_kernel(const NormArgs g) {
         if (live && t == 0)
             g.scale[row] = (float)largest < kInf ? (float)((double)largest / 127.0 * (double)rstd)
                                                  : __int_as_float(0x7fc00000);
+        // fp16 has no such products; a bf16 row whose products are all 0 in fp32 may have
+        // some in 64 bits unless it is 0 itself (the rows that pad a batch)
+        if constexpr (!std::is_same<T, __half>::value) {
+            const float m32 = (float)largest;
+            bool odd = live && !(m32 >= kTiny && m32 <= kHuge) && !(kExact64 && m32 == 0.0f && largest == (L)0);
+            if (TPR > 32 ? odd : __any_sync(0xffffffffu, odd)) {
+                if constexpr (!kExact64) odd = odd && seen != 0;
+                if (kExact64 || (TPR > 32 ? __syncthreads_or(odd) : __any_sync(0xffffffffu, odd)))
+                    products_to_8_bits<T, E, TPR, kMode>(g, opaque(row), rstd);
+            }
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < E; i += 8) {

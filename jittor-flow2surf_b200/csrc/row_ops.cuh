@@ -128,6 +128,16 @@ struct Held {
             }
         }
     }
+    // 0 where all values are 0.
+    __device__ __forceinline__ uint32_t magnitudes() const {
+        uint32_t u = 0;
+#pragma unroll
+        for (int i = 0; i < (kPacked ? E / 2 : E); ++i) {
+            if constexpr (kPacked) u |= w[i];
+            else u |= __float_as_uint(f[i]);
+        }
+        return u & (kPacked ? 0x7fff7fffu : 0x7fffffffu);
+    }
     // Values rounded to T.
     __device__ __forceinline__ void set(int i, const float (&v)[8]) {
 #pragma unroll
@@ -280,6 +290,14 @@ __device__ __forceinline__ float half_side(float v, float m, float c) {
 __device__ __forceinline__ double half_side(double v, double m, float c) {
     const double p = __dmul_rn(254.0, v), q = __dmul_rn((double)c, m);
     return __dadd_rn(__dsub_rn(p, q), __dsub_rn(__fma_rn(254.0, v, -p), __fma_rn((double)c, m, -q)));
+}
+
+// 127 v / m of such products to the nearest whole number, m finite and above 0.
+__device__ __forceinline__ int nearest_whole(double v, double m) {
+    const float below = (float)floor(127.0 * v / m);  // or, next to a whole number, the one beside it
+    const double side = half_side(v, m, 2.0f * below + 1.0f);
+    const int k = (int)below;
+    return side > 0 || (side == 0 && (k & 1)) ? k + 1 : k;
 }
 
 __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {

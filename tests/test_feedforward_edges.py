@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import flow2surf_b200 as f2s
+from test_feedforward import NORM, U, close, nearest_whole, norm64, normal, row_max
 
 # fp32 streams and weights s, w of 24 bits with 254 s1 w1 - c s0 w0 = r for c odd:
 # 127 p / m is r / (2 m) off the half c / 2, less than 64-bit products tell (they
@@ -30,7 +31,7 @@ NEXT_TO_HALVES = [
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shift", [0, -20, 38])
+@pytest.mark.parametrize("shift", [0, -20, -90, 38])
 @pytest.mark.parametrize("width", [2, 8, 200, 5000])
 def test_norm_int8_of_products_next_to_halves(cuda, width, shift):
     """The exact quotient decides, whatever power of two the products carry."""
@@ -43,3 +44,60 @@ def test_norm_int8_of_products_next_to_halves(cuda, width, shift):
         values = f2s.add_rms_norm_int8(x.to(cuda), w.to(cuda))[0].values
         q = (c + 1) // 2 if r > 0 else c // 2
         assert values[1:, :2].tolist() == [[127, q], [127, -q]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [24, 192, 191, 1530, 4096, 16391])
+@pytest.mark.parametrize("loud", [1e15, 1e30, 8.0, 1e-10, 1e-20, 1e-33])
+def test_norm_int8_of_products_that_leave_fp32(cuda, loud, width, dtype):
+    """Finite rows whose products s w lie beyond fp32 at either end, among ordinary
+    ones: each keeps its exact rounding, and a scale of its own."""
+    sizes = torch.tensor([1.0, 3e37, 1e-25, 1e25, 1e-30, 1.0, 1e10, 1e-37, 1e20])
+    x = normal(9, width, seed=width).clamp(-5, 5) * sizes[:, None]
+    x[5] = 0
+    x = x.to(dtype).to(cuda)
+    w = normal(width, dtype=dtype, seed=1, scale=loud).to(cuda)
+    rows = [0, 1, 2, 3, 4, 6, 7, 8]
+    for eps in (0.0, 1e-6):
+        for r in (None, torch.zeros_like(x)):
+            _, s, w64, rstd = norm64(x, w, r, eps)
+            p = s * w64
+            eight, _ = f2s.add_rms_norm_int8(x, w, r, eps=eps)
+            assert torch.equal(eight.values, nearest_whole(p, row_max(p)))
+            scale = (row_max(p) * rstd / 127)[:, 0]
+            close(eight.scale[rows], scale[rows], scale[rows] * (NORM + 2) * U + 1e-45)
+            assert eps == 0 or eight.scale[5] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_int8_of_halves_below_the_smallest_normal(cuda, dtype):
+    """Products of few bits that all lie below 2^-141, where exact halves are common."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randint(-255, 256, (60, 2048), generator=g).to(dtype) * 2.0**-82
+    w = torch.randint(1, 256, (2048,), generator=g).to(dtype) * 2.0**-70
+    p = x.double() * w.double()
+    twice = 254 * p / row_max(p)
+    assert ((twice == twice.round()) & (twice.remainder(2) == 1)).sum() > 10  # halves are there
+    values = f2s.add_rms_norm_int8(x.to(cuda), w.to(cuda))[0].values
+    assert torch.equal(values.cpu(), nearest_whole(p, row_max(p)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [24, 192, 4096])
+def test_norm_int8_of_rows_that_are_not_finite_beside_large_products(cuda, width, dtype):
+    x = normal(8, width, dtype=dtype, seed=1).to(cuda)
+    x[1] *= 1e25
+    x[2, 3], x[3, 0], x[4] = float("nan"), float("inf"), 0.0
+    w = normal(width, dtype=dtype, seed=2, scale=1e15).to(cuda)
+    w[0] = 0  # an infinite value times it is none
+    eight, _ = f2s.add_rms_norm_int8(x, w)
+    assert torch.isnan(eight.scale[2:4]).all() and not eight.values[2:5].any() and eight.scale[4] == 0
+    keep = [0, 1, 5, 6, 7]
+    p = x[keep].double() * w.double()
+    assert torch.equal(eight.values[keep], nearest_whole(p, row_max(p))) and torch.isfinite(eight.scale[keep]).all()
+    x[2, 3] = x[3, 0] = 0
+    none, _ = f2s.add_rms_norm_int8(x, torch.zeros_like(w))
+    assert not none.values.any() and not none.scale.any()
