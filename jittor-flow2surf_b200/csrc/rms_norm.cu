@@ -36,38 +36,25 @@ struct NormArgs {
     float* scale;
 };
 
-// This thread's part of a row's sum of squares, with its values multiplied by `up`.
-// Almost no row needs it: it reads the row again, as a call of its own, so that it
-// takes no registers from the others (from the row that is held, 300 x 8,192 with
-// 8-bit rows took 6.7 us, not 6.0; single values, which leave registers free, are
-// taken from there: 65,536 x 191 36 us, not 41).
-template <typename S, typename T>
-__device__ __noinline__ float scaled_sum(const T* s, int C, int t, float up) {
-    float sum = 0.0f;
-#pragma unroll 1
-    for (int i = 0; i < S::kEach; ++i) {
-        const int c = S::channel(i, t);
-        if (c >= C) break;
-        const float a = to_f32<T>(s[c]) * up;
-        sum = fmaf(a, a, sum);
-    }
-    return sum;
-}
-
 // The row, so that what follows from it is computed anew.
 __device__ __forceinline__ int64_t opaque(int64_t row) {
     asm volatile("" : "+l"(row));
     return row;
 }
 
-// A row whose largest product s w lies outside of [1e-30, 1e30], to 8 bits: products
-// beyond 3.4e38 are infinite in fp32 and those below 1.2e-38 lose bits, so they are
-// taken in 64 bits, which hold every one of them exactly. Almost no row needs it: it
-// reads the row and the weight again, value by value, in a call of its own that is given
-// the row's number alone, so that it takes no registers from the others.
-template <typename T, int E, int TPR, Mode kMode>
-__device__ __noinline__ void products_to_8_bits(const NormArgs& g, int64_t row, float rstd) {
+// A row that fp32 does not carry, in 64 bits, which hold every square and product of two
+// fp32 values: one whose squares leave fp32 (magnitudes above 1e18, or tiny ones with an
+// eps that does not hide them: the reciprocal root of a subnormal row is past 3.4e38
+// itself), or, for 8-bit rows, one whose largest product s w lies outside of
+// [1e-30, 1e30] (beyond 3.4e38 products are infinite in fp32, below 1.2e-38 they lose
+// bits). Almost no row is one: it is written again, value by value, after the kernel has
+// written it as any other, in a call of its own that is given the row's number alone, so
+// that it takes no registers from the others.
+template <typename T, int E, int TPR, Mode kMode, bool k8>
+__device__ __noinline__ void row_in_64_bits(const NormArgs& g, int64_t row) {
     using S = Slice<T, E, TPR, kMode>;
+    __shared__ double shared_a[32];
+    __shared__ unsigned long long shared_m[32];
     const int t = TPR <= 32 ? threadIdx.x % TPR : threadIdx.x;
     const bool live = row < g.nrows;
     const int C = live ? g.C : 0;
@@ -76,29 +63,32 @@ __device__ __noinline__ void products_to_8_bits(const NormArgs& g, int64_t row, 
     const T* s = g.residual ? static_cast<const T*>(g.stream) + row * (int64_t)g.C
                             : static_cast<const T*>(g.x) + row * g.ldx;
     const T* w = static_cast<const T*>(g.weight);
-    int8_t* q = g.q + row * g.ldq;
-    __shared__ unsigned long long shared_m[32];
-    float none = 0.0f;
+    double sum = 0.0;
     unsigned long long bits = 0;
 #pragma unroll 1
     for (int i = 0; i < S::kEach; ++i) {
         const int c = S::channel(i, t);
         if (c >= C) break;
-        const double p = fabs((double)to_f32<T>(s[c]) * (double)to_f32<T>(w[c]));
-        const unsigned long long b = (unsigned long long)__double_as_longlong(p);
-        bits = b > bits ? b : bits;
+        const double a = (double)to_f32<T>(s[c]);
+        sum = fma(a, a, sum);
+        if constexpr (k8) {
+            const auto p = (unsigned long long)__double_as_longlong(fabs(a * (double)to_f32<T>(w[c])));
+            bits = p > bits ? p : bits;
+        }
     }
-    row_sum_max<TPR, false, true>(none, bits, &none, shared_m);
+    row_sum_max<TPR, true, k8>(sum, bits, shared_a, shared_m);
+    const double rstd = 1.0 / sqrt(sum / (double)g.C + (double)g.eps);
     const double m = __longlong_as_double((long long)bits);
     const bool finite = m < (double)kInf;
 #pragma unroll 1
     for (int i = 0; i < S::kEach; ++i) {
         const int c = S::channel(i, t);
         if (c >= C) break;
-        const double p = (double)to_f32<T>(s[c]) * (double)to_f32<T>(w[c]);
-        q[c] = (int8_t)(finite && m > 0.0 ? nearest_whole(p, m) : 0);
+        const double a = (double)to_f32<T>(s[c]), b = (double)to_f32<T>(w[c]);
+        if constexpr (k8) g.q[row * g.ldq + c] = (int8_t)(finite && m > 0.0 ? nearest_whole(a * b, m) : 0);
+        else static_cast<T*>(g.y)[row * (int64_t)g.C + c] = from_f32<T>((float)(a * rstd * b));
     }
-    if (live && t == 0) g.scale[row] = finite ? (float)(m / 127.0 * (double)rstd) : __int_as_float(0x7fc00000);
+    if (k8 && live && t == 0) g.scale[row] = finite ? (float)(m / 127.0 * rstd) : __int_as_float(0x7fc00000);
 }
 
 // 8 single bf16 values with 8-bit rows stay at 48 registers for a fifth 256-thread
@@ -172,23 +162,8 @@ add_rms_norm_kernel(const __grid_constant__ NormArgs g) {
         if constexpr (k8 && !kExact64) m = max_abs(b, m);
     }
     row_sum_max<TPR, true, k8>(sum, m, shared_a, shared_m);
-    float rstd;
-    const float up = square_scale(sum, g.eps);
-    if (sums_again<T, TPR>(up)) {
-        if constexpr (kMode == kSingle) {
-            sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < E; ++i) sum = fmaf(s.f[i] * up, s.f[i] * up, sum);
-        } else {
-            sum = scaled_sum<S>(from, C, t, up);
-        }
-        if (TPR > 32) __syncthreads();  // the first sum has been read
-        M none = 0;
-        row_sum_max<TPR, true, false>(sum, none, shared_a, shared_m);
-        rstd = reciprocal_rms(sum, g.C, g.eps * up * up) * up;
-    } else {
-        rstd = reciprocal_rms(sum, g.C, g.eps);
-    }
+    const float rstd = reciprocal_rms(sum, g.C, g.eps);
+    bool odd = live && squares_leave_fp32(sum, g.eps), some = odd;
     if constexpr (k8) {
         using L = typename std::conditional<kExact64, double, float>::type;
         L largest;
@@ -217,17 +192,12 @@ add_rms_norm_kernel(const __grid_constant__ NormArgs g) {
         if (live && t == 0)
             g.scale[row] = (float)largest < kInf ? (float)((double)largest / 127.0 * (double)rstd)
                                                  : __int_as_float(0x7fc00000);
-        // fp16 has no such products; a bf16 row whose products are all 0 in fp32 may have
-        // some in 64 bits unless it is 0 itself (the rows that pad a batch)
-        if constexpr (!std::is_same<T, __half>::value) {
-            const float m32 = (float)largest;
-            bool odd = live && !(m32 >= kTiny && m32 <= kHuge) && !(kExact64 && m32 == 0.0f && largest == (L)0);
-            if (TPR > 32 ? odd : __any_sync(0xffffffffu, odd)) {
-                if constexpr (!kExact64) odd = odd && seen != 0;
-                if (kExact64 || (TPR > 32 ? __syncthreads_or(odd) : __any_sync(0xffffffffu, odd)))
-                    products_to_8_bits<T, E, TPR, kMode>(g, opaque(row), rstd);
-            }
-        }
+        const bool outside = live && !((float)largest >= kTiny && (float)largest <= kHuge);
+        // a row without products needs no more, one of the rows that pad a batch; where
+        // they are 0 in fp32 alone, some of its values are not 0
+        some = kExact64 ? largest != (L)0 : largest != (L)0 || seen != 0;
+        some = odd || (outside && some);
+        odd = odd || outside;
     } else {
 #pragma unroll
         for (int i = 0; i < E; i += 8) {
@@ -239,6 +209,13 @@ add_rms_norm_kernel(const __grid_constant__ NormArgs g) {
             s.set(i, a);
         }
         store_held<TPR>(static_cast<T*>(g.y) + at * (int64_t)g.C, C, t, s);
+    }
+    // fp16 has neither such squares nor such products
+    if constexpr (!std::is_same<T, __half>::value) {
+        // all threads of a row of several warps agree on `odd`, not on `some`
+        bool again = TPR > 32 ? odd : __any_sync(0xffffffffu, odd);
+        if (k8 && again) again = TPR > 32 ? __syncthreads_or(some) : __any_sync(0xffffffffu, some);
+        if (again) row_in_64_bits<T, E, TPR, kMode, k8>(g, opaque(row));
     }
 }
 

@@ -67,7 +67,8 @@ __device__ void rows_again(const NormGradArgs& g, int rows_at_once, float* share
             float m = 0.0f, sum = 0.0f, along = 0.0f;
             for (int c = threadIdx.x; c < g.C; c += threads) m = max_abs(m, m, to_f32<T>(s[c]));
             m = join(m, shared_a, true);
-            const float by = square_scale(m * m * (float)g.C, g.eps);  // C m^2 bounds the sum
+            const float most = m * m * (float)g.C;  // bounds the sum
+            const float by = !squares_leave_fp32(most, g.eps) ? 1.0f : most > 1.0f ? 0x1p-80f : 0x1p100f;
             for (int c = threadIdx.x; c < g.C; c += threads) {
                 const float a = to_f32<T>(s[c]) * by;
                 sum = fmaf(a, a, sum);
@@ -75,11 +76,12 @@ __device__ void rows_again(const NormGradArgs& g, int rows_at_once, float* share
             }
             sum = join(sum, shared_a, false);
             along = join(along, shared_b, false);
-            const float norm = reciprocal_rms(sum, g.C, g.eps * by * by), rstd = norm * by;
+            // the reciprocal root is norm by, which may leave fp32 where the row is tiny
+            const float norm = reciprocal_rms(sum, g.C, g.eps * by * by);
             const float mean = along * norm / (float)g.C;
             for (int c = threadIdx.x; c < g.C; c += threads) {
-                const float d = to_f32<T>(dy[c]), n = to_f32<T>(s[c]) * rstd;
-                float grad = rstd * (d * to_f32<T>(w[c]) - n * mean);
+                const float d = to_f32<T>(dy[c]), n = to_f32<T>(s[c]) * by * norm;
+                float grad = norm * (d * to_f32<T>(w[c]) - n * mean) * by;
                 if (ds) grad += to_f32<T>(ds[c]);
                 dx[c] = from_f32<T>(grad);
                 if (mine) mine[c] = fmaf(d, n, mine[c]);
@@ -156,7 +158,7 @@ add_rms_norm_grad_kernel(const NormGradArgs g) {
             along = lanes_sum<kWarps>(shared_b[parity][lane % kWarps]);
             parity ^= 1;
         }
-        again = again || (live && square_scale(sum, g.eps) != 1.0f);
+        again = again || (live && squares_leave_fp32(sum, g.eps));
         // 0 past the last row: with eps = 0 its reciprocal would put NaN into dw
         const float rstd = live ? reciprocal_rms(sum, g.C, g.eps) : 0.0f;
         const float mean = along * rstd / (float)g.C;  // mean(u n)

@@ -229,8 +229,8 @@ __device__ __forceinline__ unsigned long long lanes_max(unsigned long long m) {
     }
     return m;
 }
-template <int TPR>
-__device__ __forceinline__ float lanes_sum(float a) {
+template <int TPR, typename A>
+__device__ __forceinline__ A lanes_sum(A a) {
 #pragma unroll
     for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     return a;
@@ -239,8 +239,8 @@ __device__ __forceinline__ float lanes_sum(float a) {
 // Sum of `a` (kSum) and maximum of `m` (kMax) over the TPR threads of a row;
 // every thread gets both. The shared arrays hold TPR / 32 entries for TPR > 32;
 // two uses need a barrier between them.
-template <int TPR, bool kSum, bool kMax, typename M>
-__device__ __forceinline__ void row_sum_max(float& a, M& m, float* shared_a, M* shared_m) {
+template <int TPR, bool kSum, bool kMax, typename A, typename M>
+__device__ __forceinline__ void row_sum_max(A& a, M& m, A* shared_a, M* shared_m) {
     if constexpr (kSum) a = lanes_sum<TPR>(a);
     if constexpr (kMax) m = lanes_max<TPR>(m);
     if constexpr (TPR > 32) {
@@ -449,19 +449,11 @@ __device__ __forceinline__ void widen8(uint32_t w, float* v) {
     v[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - 8388736.0f;
 }
 
-// What a row's values are multiplied by before their squares are summed again,
-// where the sum of the squares themselves is outside of what fp32 holds well (rows
-// of magnitudes above 1e18, or below 1e-14 with an eps that does not hide them).
-// fp16 has no values of the first kind and its squares are never below 2^-48.
-__device__ __forceinline__ float square_scale(float sum, float eps) {
-    return sum > 0x1p120f ? 0x1p-80f : sum < 0x1p-90f && eps < 0x1p-90f ? 0x1p100f : 1.0f;
-}
-// Whether to do that: true for all of the threads that share a row or a warp.
-template <typename T, int TPR>
-__device__ __forceinline__ bool sums_again(float scale) {
-    if constexpr (std::is_same<T, __half>::value) return false;
-    else if constexpr (TPR < 32) return __any_sync(0xffffffffu, scale != 1.0f);
-    else return scale != 1.0f;
+// Whether a row's sum of squares is outside of what fp32 holds well: rows of
+// magnitudes above 1e18, or below 1e-14 with an eps that does not hide them. fp16 has no
+// values of the first kind and its squares are never below 2^-48.
+__device__ __forceinline__ bool squares_leave_fp32(float sum, float eps) {
+    return sum > 0x1p120f || (sum < 0x1p-90f && eps < 0x1p-90f);
 }
 
 // Reciprocal root of a row's mean square from its sum.

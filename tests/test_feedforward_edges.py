@@ -10,7 +10,8 @@ import pytest
 import torch
 
 import flow2surf_b200 as f2s
-from test_feedforward import NORM, U, close, nearest_whole, norm64, normal, row_max
+from test_feedforward import (DEPTH, NORM, U, close, half_step, nearest_whole, norm64, norm_grad64, normal, row_max,
+                              smallest)
 
 # fp32 streams and weights s, w of 24 bits with 254 s1 w1 - c s0 w0 = r for c odd:
 # 127 p / m is r / (2 m) off the half c / 2, less than 64-bit products tell (they
@@ -101,3 +102,43 @@ def test_norm_int8_of_rows_that_are_not_finite_beside_large_products(cuda, width
     x[2, 3] = x[3, 0] = 0
     none, _ = f2s.add_rms_norm_int8(x, torch.zeros_like(w))
     assert not none.values.any() and not none.scale.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [24, 192, 191, 1530, 4096, 16391])
+@pytest.mark.parametrize("sizes", [(1e-40, 1e-39, 1e-41), (3e-40, 1e-39, 2e-39)])
+def test_norm_of_rows_whose_reciprocal_leaves_fp32(cuda, sizes, width, dtype):
+    """Subnormal rows with eps 0: their reciprocal root is past 3.4e38, the normed
+    rows and the weight's gradient are of order 1. A row that is 0 in bf16 (its
+    smallest value is 9e-41) has none of them: 0 / 0."""
+
+    def close_or_none(got, want, bound):
+        none = torch.isnan(want)
+        assert torch.equal(torch.isnan(got), none)
+        close(got[~none], want[~none], bound[~none])
+
+    x = normal(9, width, dtype=dtype, seed=width)
+    x[[1, 4, 5]] = (x[[1, 4, 5]] * torch.tensor(sizes)[:, None]).to(dtype)
+    x = x.to(cuda).requires_grad_()
+    w = normal(width, dtype=dtype, seed=1).to(cuda).requires_grad_()
+    dy = normal(9, width, dtype=dtype, seed=2).to(cuda)
+    dy[[1, 4, 5]] *= 1e-9  # so that dx is finite
+    _, s, w64, rstd = norm64(x.detach(), w.detach(), None, 0.0)
+    assert (rstd > 3.5e38).sum() >= 1
+    y, _ = f2s.add_rms_norm(x, w, eps=0.0)
+    y64 = s * rstd * w64
+    close_or_none(y.detach(), y64, y64.abs() * (half_step(dtype) + NORM * U) * 1.001 + smallest(dtype))
+    with torch.no_grad():
+        eight, _ = f2s.add_rms_norm_int8(x, w, eps=0.0)
+    p = s * w64
+    assert torch.equal(eight.values, nearest_whole(p, row_max(p)))
+    scale = (row_max(p) * rstd / 127)[:, 0]
+    close_or_none(eight.scale, scale, scale * (NORM + 2) * U)
+    got_dx, got_dw = torch.autograd.grad(y, (x, w), dy)
+    dx, dw, (rstd, u, n) = norm_grad64(x.detach(), w.detach(), dy, None, 0.0)
+    mean = (u * n).abs().mean(-1, keepdim=True)
+    bound = half_step(dtype) * dx.abs() + U * (rstd * ((NORM + 4) * u.abs() + (DEPTH + 3 * NORM + 6) * n.abs() * mean))
+    close_or_none(got_dx, dx, bound * 1.001 + smallest(dtype))
+    terms = (dy.double() * n).abs().sum(0)
+    close_or_none(got_dw, dw, half_step(dtype) * dw.abs() + U * (9 + NORM + 1) * terms + smallest(dtype))
