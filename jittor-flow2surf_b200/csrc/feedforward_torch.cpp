@@ -7,6 +7,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros_like.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -73,6 +74,15 @@ bool needs_grad(std::initializer_list<const Tensor*> tensors) {
     for (const Tensor* t : tensors)
         if (t && t->defined() && t->requires_grad()) return true;
     return false;
+}
+
+// Tangents of forward-mode differentiation, which would be lost (and read as zeros):
+// they come with or without requires_grad, and torch.no_grad() leaves them on.
+void refuse_tangents(std::initializer_list<const Tensor*> tensors) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_VALUE(!(t && t->defined() && t->_fw_grad(/*level=*/0).defined()),
+                          "the 8-bit feed-forward operators have no forward-mode derivative");
 }
 
 // A (..., channels) tensor read as rows of one pitch: as it is where its last
@@ -143,6 +153,7 @@ void check_eight(const char* name, const Tensor& values, const Tensor& scale) {
 std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
     check_rows("x", x);
     const int code = dtype_code(x.scalar_type());
+    refuse_tangents({&x});
     check_device(x, {});
     TORCH_CHECK_VALUE(!needs_grad({&x}), "8-bit rows have no gradient; call quantize_rows under torch.no_grad()");
     Eight out = empty_eight(x, x.size(-1));
@@ -156,6 +167,7 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
 
 Tensor dequantize_rows(const Tensor& values, const Tensor& scale, at::ScalarType type) {
     const int code = dtype_code(type);
+    refuse_tangents({&scale});
     check_eight("rows", values, scale);
     Tensor out = at::empty(values.sizes(), values.options().dtype(type));
     if (out.numel() == 0) return out;
@@ -171,6 +183,7 @@ Tensor dequantize_rows(const Tensor& values, const Tensor& scale, at::ScalarType
 Tensor linear_int8(const Tensor& xv, const Tensor& xs, const Tensor& wv, const Tensor& ws,
                    const optional<Tensor>& bias, at::ScalarType type) {
     const int code = dtype_code(type);
+    refuse_tangents({&xs, &ws, bias ? &*bias : nullptr});
     check_eight("x", xv, xs);
     check_eight("weight", wv, ws);
     TORCH_CHECK_VALUE(wv.dim() == 2, "weight must be (cols, K), got ", shape_of(wv));
@@ -209,6 +222,7 @@ int check_norm(const Tensor& x, const Tensor& weight, const Tensor& residual) {
                       "residual must be ", shape_of(x), " of ", c10::toString(x.scalar_type()), ", got ",
                       residual.defined() ? shape_of(residual) : "", " of ",
                       residual.defined() ? c10::toString(residual.scalar_type()) : "");
+    refuse_tangents({&x, &weight, &residual});
     check_device(x, {&weight, &residual});
     return code;
 }
@@ -333,6 +347,7 @@ int check_projected(const Tensor& p) {
     check_rows("projected", p);
     TORCH_CHECK_VALUE(p.size(-1) % 2 == 0, "projected must be (..., 2 H) = [gate | value], got ", shape_of(p));
     const int code = dtype_code(p.scalar_type());
+    refuse_tangents({&p});
     check_device(p, {});
     return code;
 }

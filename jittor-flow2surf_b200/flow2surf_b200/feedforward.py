@@ -11,7 +11,8 @@ arithmetic is fp32. A last dimension of stride 1 whose rows lie at one pitch is
 taken as it is, other layouts are copied first. Calls run on the current stream
 of the tensors' device, may be captured into CUDA graphs, and keep nothing
 between one another. Arguments that do not fit raise ValueError. There is no CPU
-path, and no second derivative.
+path, no second derivative, and no forward-mode one (tensors with a tangent are
+refused).
 
 The checks, outputs and autograd nodes are native (csrc/feedforward_torch.cpp):
 in Python they take longer than the kernels of a decode step.

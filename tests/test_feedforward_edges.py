@@ -8,8 +8,10 @@ exact quotient.
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flow2surf_b200 as f2s
+from flow2surf_b200.feedforward import Int8Rows
 from test_feedforward import (DEPTH, NORM, U, close, half_step, nearest_whole, norm64, norm_grad64, normal, row_max,
                               smallest)
 
@@ -142,3 +144,40 @@ def test_norm_of_rows_whose_reciprocal_leaves_fp32(cuda, sizes, width, dtype):
     close_or_none(got_dx, dx, bound * 1.001 + smallest(dtype))
     terms = (dy.double() * n).abs().sum(0)
     close_or_none(got_dw, dw, half_step(dtype) * dw.abs() + U * (9 + NORM + 1) * terms + smallest(dtype))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """On the host, before anything else of the call: no output without its tangent."""
+    plain = torch.ones(4, 8)
+    w, eight = torch.ones(8), Int8Rows(torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4))
+    with forward_ad.dual_level():
+        for grad in (False, True):
+            x = forward_ad.make_dual(plain.clone().requires_grad_(grad), torch.ones(4, 8))
+            dual_w = forward_ad.make_dual(w.clone().requires_grad_(grad), w)
+            scale = forward_ad.make_dual(torch.ones(4).requires_grad_(grad), torch.ones(4))
+            learnt = Int8Rows(eight.values, scale)
+            calls = [lambda: f2s.add_rms_norm(x, w), lambda: f2s.add_rms_norm(plain, dual_w),
+                     lambda: f2s.add_rms_norm(plain, w, x), lambda: f2s.add_rms_norm_int8(plain, w, x),
+                     lambda: f2s.swiglu(x), lambda: f2s.swiglu(x, checkpoint="int8"), lambda: f2s.swiglu_int8(x),
+                     lambda: f2s.quantize_rows(x), lambda: learnt.dequantize(), lambda: f2s.linear_int8(learnt, eight),
+                     lambda: f2s.linear_int8(eight, learnt),
+                     lambda: f2s.linear_int8(eight, eight, scale, dtype=torch.float32)]
+            for call in calls:
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                    call()
+        primal = forward_ad.unpack_dual(x).primal
+        with pytest.raises(ValueError, match="CUDA tensors"):  # without its tangent it is an ordinary one
+            f2s.swiglu(primal)
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_on_the_device_are_refused(cuda):
+    x, w = normal(4, 64, seed=1).to(cuda), normal(64, seed=2).to(cuda)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda t: f2s.add_rms_norm(t, w), lambda t: f2s.swiglu(t), lambda t: f2s.quantize_rows(t)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(dual)
+            call(x)
