@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _f32, _needs_grad, _require_cuda
+from .ops import _f32, _needs_grad, _refuse_tangents, _require_cuda
 
 
 def _dcd_call(pred, target, alpha, grad_loss=None, want_grads=False):
@@ -60,6 +60,7 @@ def dcd_loss(pred: torch.Tensor, target: torch.Tensor, alpha: float) -> torch.Te
         raise ValueError(f"Batch sizes differ: {pred.shape[0]} and {target.shape[0]}")
     if pred.shape[1] < 1 or target.shape[1] < 1:
         raise ValueError("Point sets must be nonempty")
+    _refuse_tangents(pred, target)
     _require_cuda(pred, target)
     if _needs_grad(pred, target):
         return _DcdLoss.apply(pred, target, float(alpha))
@@ -101,6 +102,7 @@ def velocity_loss(pred_velocity: torch.Tensor, target_velocity: torch.Tensor) ->
     if pred_velocity.shape != target_velocity.shape or pred_velocity.dim() != 3:
         raise ValueError(f"velocities must share a (B, M, 3) shape, got "
                          f"{tuple(pred_velocity.shape)} and {tuple(target_velocity.shape)}")
+    _refuse_tangents(pred_velocity, target_velocity)
     _require_cuda(pred_velocity, target_velocity)
     if _needs_grad(pred_velocity, target_velocity):
         return _VelocityLoss.apply(pred_velocity, target_velocity)

@@ -11,8 +11,17 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
+
+
+def _refuse_tangents(*tensors):
+    """Of forward-mode differentiation: they would be lost, and read as zeros."""
+    if forward_ad._current_level < 0:  # as unpack_dual asks: there are no tangents
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("flow2surf_b200 operators have no forward-mode derivative")
 
 
 def _require_cuda(*tensors):
@@ -78,6 +87,7 @@ def offset_attention_aggregate(query: torch.Tensor, key: torch.Tensor,
             or query.shape[2] != key.shape[1]):
         raise ValueError(f"Incompatible attention shapes: {tuple(query.shape)}, "
                          f"{tuple(key.shape)}, {tuple(value.shape)}")
+    _refuse_tangents(query, key, value)
     _require_cuda(query, key, value)
     if _needs_grad(query, key, value):
         if precision != "fp32":
@@ -172,6 +182,7 @@ def reduce_neighbor_messages(content, geometry, indices, hpe_input_weight, hpe_i
     tensors = (content, geometry, indices, hpe_input_weight, hpe_input_bias, hpe_output_weight,
                hpe_output_bias, hpe_norm_weight, hpe_norm_bias, message_norm_weight,
                message_norm_bias)
+    _refuse_tangents(*tensors)
     _require_cuda(*tensors)
     if _needs_grad(*tensors):
         return _NeighborMessages.apply(precision, *tensors)
@@ -305,6 +316,7 @@ def nearest_squared_distances(first: torch.Tensor, second: torch.Tensor):
         raise ValueError("Point sets must be nonempty")
     if first.dtype != second.dtype:
         raise ValueError(f"Dtypes differ: {first.dtype} and {second.dtype}")
+    _refuse_tangents(first, second)
     _require_cuda(first, second)
     if _needs_grad(first, second):
         return _NearestDistance.apply(first, second)
