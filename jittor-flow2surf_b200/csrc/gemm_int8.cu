@@ -70,6 +70,10 @@ __device__ __forceinline__ void store_cluster(uint32_t a, uint32_t x, uint32_t y
                  : "memory");
 }
 
+__device__ __forceinline__ void store_cluster(uint32_t a, uint32_t x) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ float bias_at(const void* bias, int n) {
     return bias ? to_f32<T>(static_cast<const T*>(bias)[n]) : 0.0f;
@@ -105,6 +109,8 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     uint64_t* empty = full + S;
     uint64_t* done = empty + S;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // K blocks loaded,
+    int* used = issued + 1;                               // and multiplied
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = g.split;
@@ -142,21 +148,19 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
 
     if (warp == 0) {
         if (lane == 0) {
-            for (int i = ahead; i < blocks; ++i) {
-                if (i >= S && !wait_poll(&empty[i % S], ((uint32_t)(i / S) & 1u) ^ 1u, g.err)) {
-                    // let the copies already issued land before the CTA exits:
-                    // each stage's last one
-                    for (int j = i - S; j < i; ++j) tc::mbar_drain(&full[j % S], (uint32_t)(j / S) & 1u);
-                    break;
-                }
+            int i = ahead;
+            for (; i < blocks; ++i) {
+                if (i >= S && !wait_poll(&empty[i % S], ((uint32_t)(i / S) & 1u) ^ 1u, g.err)) break;
                 load(i);
             }
+            *issued = i;
         }
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const int i = kb - kb0, s = i % S;
+            int i = 0;
+            for (; i < blocks; ++i) {
+                const int s = i % S;
                 if (!wait_poll(&full[s], (uint32_t)(i / S) & 1u, g.err)) break;
                 tc::tc_fence_after();
                 const uint32_t st = tc::smem_u32(smem + (size_t)s * kStage);
@@ -166,6 +170,7 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
                     umma_i8(tmem, a + 2 * k, b + 2 * k, idesc_i8(128, BN), (i | k) ? 1u : 0u);
                 tc::umma_commit(&empty[s]);
             }
+            *used = i;
             // every MMA issued has completed (TMEM is freed below)
             tc::umma_commit(done);
             tc::mbar_drain(done, 0);
@@ -205,6 +210,11 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     __syncthreads();
     tc::tc_fence_after();
     if (warp == 1) tc::tmem_dealloc(tmem, kCols);
+    // where a wait ran out, the copies still under way land before the CTA exits
+    auto land = [&]() {
+        if (threadIdx.x == 0)
+            for (int i = *used; i < *issued; ++i) tc::mbar_drain(&full[i % S], (uint32_t)(i / S) & 1u);
+    };
 
     auto store = [&](int m, int acc) {
         static_cast<T*>(g.y)[m * g.ldy + n] = from_f32<T>(fmaf((float)acc * __ldg(g.xs + m), ws, b));
@@ -215,6 +225,7 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
             for (int j = 0; j < BN; ++j)
                 if (m0 + j < g.rows) store(m0 + j, (int)v[j]);
         }
+        land();
         return;
     }
     cluster_wait();
@@ -231,6 +242,7 @@ linear_int8_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid
     }
     cluster_arrive();
     cluster_wait();
+    land();
     if (warp < 2 || !ok || n >= g.cols) return;
     for (int four = rank; four < BN / 4; four += split) {
         const int m = m0 + four * 4;
@@ -385,6 +397,21 @@ __device__ __forceinline__ void arrive_pair(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// K blocks `used` to `loaded` or `other` are loaded by the leader or the other CTA, at
+// most one of each stage, and not waited for: until they land. A barrier counts both
+// CTAs' bytes; a part that one of them no longer loaded is taken off, or not expected.
+__device__ __forceinline__ void drain_pair(uint64_t* full, int S, uint32_t stage_bytes, int used, int loaded, int other) {
+    for (int i = used; i < loaded || i < other; ++i) {
+        uint64_t* bar = &full[i % S];
+        if (i >= other)
+            asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(tc::smem_u32(bar)),
+                         "r"(stage_bytes)
+                         : "memory");
+        if (i >= loaded) tc::mbar_arrive_expect_tx(bar, stage_bytes);
+        tc::mbar_drain(bar, (uint32_t)(i / S) & 1u);
+    }
+}
+
 // 16 lanes x 64 columns of TMEM: register 4 j + 2 i + k holds lane t / 4 + 8 i of
 // column 8 j + 2 (t % 4) + k, for thread t.
 __device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[32]) {
@@ -440,6 +467,8 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     uint64_t* tempty = tfull + 2;  // [2] leader's: eight epilogue warps of both CTAs
     uint64_t* done = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // [2] leader's: K blocks that each CTA loaded
+    int* used = issued + 2;                               // leader's: and multiplied
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -476,8 +505,8 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
 
     if (warp == 0) {
         if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0, pending = 0, pending_phase = 0;
+            int stage = 0, count = 0;
+            uint32_t phase = 0;
             bool ok = true;
             for (; ok && walk.t < tiles; walk.next(g, pairs)) {
                 int m0, n0;
@@ -492,28 +521,19 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     if (rank == 0) tc::mbar_arrive_expect_tx(&full[stage], 2 * stage_bytes);
                     tma_load_pair(st, &map_x, bar, kb * kBlockK, m0 + (int)rank * 128);
                     tma_load_pair(st + a_bytes, &map_w, bar, kb * kBlockK, n0 + (int)rank * (g.bn / 2));
-                    pending |= 1u << stage;
-                    pending_phase = (pending_phase & ~(1u << stage)) | (phase << stage);
+                    ++count;
                     if (++stage == S) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
             }
-            if (!ok) {
-                // let the copies already issued land before the CTAs exit: the
-                // leader's barriers count both CTAs' bytes; a copy of the other
-                // CTA that the leader did not expect any more has a millisecond
-                if (rank == 0)
-                    for (int s = 0; s < S; ++s)
-                        if (pending & (1u << s)) tc::mbar_drain(&full[s], (pending_phase >> s) & 1u);
-                for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-            }
+            store_cluster(map_rank(tc::smem_u32(issued + rank), 0), (uint32_t)count);
         }
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
-            int stage = 0, iter = 0;
+            int stage = 0, iter = 0, count = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int t = pair; ok && t < tiles; t += pairs, ++iter) {
@@ -526,6 +546,7 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                         ok = false;
                         break;
                     }
+                    ++count;
                     tc::tc_fence_after();
                     const uint32_t st = tc::smem_u32(smem + (size_t)stage * stage_bytes);
                     const uint64_t a = tc::sw128_desc(st), b = tc::sw128_desc(st + a_bytes);
@@ -539,6 +560,7 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                 }
                 if (ok) commit_pair(&tfull[buf]);
             }
+            *used = count;
             commit_pair(done);
             tc::mbar_drain(done, 0);
         }
@@ -687,6 +709,12 @@ linear_int8_pairs_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     cluster_arrive();
     cluster_wait();
     tc::tc_fence_after();
+    // what is still under way to this CTA lands before either leaves: the arrivals of the
+    // leader's commits at the other CTA and, where a wait ran out, copies
+    if (threadIdx.x == 0) {
+        if (rank == 0) drain_pair(full, S, stage_bytes, *used, issued[0], issued[1]);
+        else tc::mbar_drain(done, 0);
+    }
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     __syncthreads();

@@ -12,8 +12,8 @@ from torch.autograd import forward_ad
 
 import flow2surf_b200 as f2s
 from flow2surf_b200.feedforward import Int8Rows
-from test_feedforward import (DEPTH, NORM, U, close, half_step, nearest_whole, norm64, norm_grad64, normal, row_max,
-                              smallest)
+from test_feedforward import (DEPTH, NORM, U, close, eighths, half_step, nearest_whole, norm64, norm_grad64, normal,
+                              row_max, smallest)
 
 # fp32 streams and weights s, w of 24 bits with 254 s1 w1 - c s0 w0 = r for c odd:
 # 127 p / m is r / (2 m) off the half c / 2, less than 64-bit products tell (they
@@ -181,3 +181,26 @@ def test_forward_mode_derivatives_on_the_device_are_refused(cuda):
             with pytest.raises(ValueError, match="forward-mode"):
                 call(dual)
             call(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,K", [(24, 515, 4096), (24, 2048, 8192), (60, 300, 2048), (300, 192, 200), (3000, 1024, 4096),
+                                         (5000, 4096, 192)])
+def test_linear_int8_beside_a_wait_that_ran_out(cuda, rows, cols, K):
+    """A wait that ran out elsewhere ends the product's waits early: nothing is
+    written beside its rows, the error is reported, and the next call is whole."""
+    x, w = eighths(rows, K, 1, cuda), eighths(cols, K, 2, cuda)
+    want = f2s.linear_int8(x, w)
+    f2s._lib.check_device_error()
+    y = torch.full((rows + 3, cols), 55.0, dtype=torch.bfloat16, device=cuda)
+    f2s._lib.call("f2s_selftest_wait_timeout", 64, f2s._lib.stream_handle())
+    for _ in range(5):
+        f2s._lib.call("f2s_linear_int8", x.values.data_ptr(), x.values.stride(0), x.scale.data_ptr(), w.values.data_ptr(),
+                      w.values.stride(0), w.scale.data_ptr(), None, y.data_ptr(), cols, 1, rows, cols, K,
+                      f2s._lib.stream_handle())
+    with pytest.raises(f2s._lib.Flow2SurfError, match="device error 1"):
+        f2s._lib.check_device_error()
+    assert (y[rows:] == 55).all()
+    for _ in range(3):
+        assert torch.equal(f2s.linear_int8(x, w), want)
+    f2s._lib.check_device_error()
