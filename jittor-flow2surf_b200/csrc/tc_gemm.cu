@@ -789,6 +789,17 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
+// The encoder needs a current context. A host thread that has made no CUDA call of that
+// kind yet has none: setting its device makes one.
+template <typename F>
+CUresult with_context(F encode) {
+    CUresult r = encode();
+    int dev = 0;
+    if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+        r = encode();
+    return r;
+}
+
 template <bool kTf32, int kEpi, bool kSplit = false, int kEW = 8>
 int launch_tc(const CUtensorMap& ma, const CUtensorMap& ma2, const CUtensorMap& mb,
               const CUtensorMap& mb2, const CUtensorMap& my, const TcGemmArgs& g, size_t smem,
@@ -832,10 +843,12 @@ int make_tensor_map_2d_typed(CUtensorMap* map, const void* base, TmaType type, i
                                    : type == kTmaBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                    : type == kTmaU8   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = with_context([&] {
+        return enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
     if (r != CUDA_SUCCESS) return fail(F2S_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return F2S_OK;
 }
@@ -868,9 +881,11 @@ int make_tensor_map_3d_typed(CUtensorMap* map, const void* base, TmaType type, i
     const CUtensorMapDataType dt = type == kTmaF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : type == kTmaBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const CUresult r = enc(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = with_context([&] {
+        return enc(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
     if (r != CUDA_SUCCESS) return fail(F2S_ERR_CUDA, "cuTensorMapEncodeTiled (3-D) failed (%d)", (int)r);
     return F2S_OK;
 }

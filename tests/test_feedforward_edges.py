@@ -6,6 +6,8 @@ test_feedforward.py; 8-bit values have to be the nearest whole numbers of the
 exact quotient.
 """
 
+import threading
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -204,3 +206,22 @@ def test_linear_int8_beside_a_wait_that_ran_out(cuda, rows, cols, K):
     for _ in range(3):
         assert torch.equal(f2s.linear_int8(x, w), want)
     f2s._lib.check_device_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [8, 600])
+def test_linear_int8_from_a_thread_without_a_context(cuda, rows):
+    """The first CUDA call of a host thread may be one of the C entry."""
+    x, w = eighths(rows, 256, 1, cuda), eighths(192, 256, 2, cuda)
+    want = f2s.linear_int8(x, w)
+    y = torch.empty_like(want)
+    torch.cuda.synchronize()
+    entry, status = f2s._lib.lib().f2s_linear_int8, []
+    args = (x.values.data_ptr(), 256, x.scale.data_ptr(), w.values.data_ptr(), 256, w.scale.data_ptr(), None, y.data_ptr(),
+            192, 1, rows, 192, 256, torch.cuda.Stream().cuda_stream)
+    thread = threading.Thread(target=lambda: status.append((entry(*args), f2s._lib.lib().f2s_last_error())))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert status[0][0] == f2s._lib.F2S_OK, status
+    assert torch.equal(y, want)
