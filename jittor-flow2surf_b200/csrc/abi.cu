@@ -28,6 +28,30 @@ int check_launch(const char* what) {
     return F2S_OK;
 }
 
+int allow_shared(const void* kernel, size_t bytes) {
+    struct Limit {
+        const void* kernel;
+        int dev;
+        size_t bytes;
+    };
+    // more than the library's kernels on one device; past it, limits are set as asked
+    constexpr int kLimits = 1024;
+    static Limit limits[kLimits];
+    static int count = 0;
+    static std::mutex mutex;
+    int dev = 0;
+    F2S_CUDA_TRY(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mutex);
+    int i = 0;
+    while (i < count && (limits[i].kernel != kernel || limits[i].dev != dev)) ++i;
+    if (i < count && limits[i].bytes > bytes) bytes = limits[i].bytes;
+    // set even where it is known, as a device that was reset has forgotten it
+    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (i == count && count < kLimits) limits[count++] = {kernel, dev, bytes};
+    else if (i < count) limits[i].bytes = bytes;
+    return F2S_OK;
+}
+
 int sm_count() {
     static std::mutex cache_mutex;
     static int cached[64] = {0};

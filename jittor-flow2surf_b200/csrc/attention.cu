@@ -196,8 +196,7 @@ int launch_output(const float* q, const float* k, int ldqk, const float* v, int 
     const size_t smem = sizeof(float) * ((size_t)TQ * dp + TK * dp + (size_t)TK * C +
                                          TQ * (TK + 1) + TK);
     auto kernel = attn_output_kernel<CJ>;
-    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)smem));
+    F2S_TRY(allow_shared(kernel, smem));
     const int tiles = ceil_div(N, TQ);
     TraceScope trace(kTagAttnOutput, stream);
     kernel<<<B * tiles, 256, smem, stream>>>(q, k, ldqk, v, ldv, L, h, ldh, out, ldo, N, d, C,
@@ -215,8 +214,7 @@ int attention_f32(const float* q, const float* k, int ldqk, const float* v, int 
     F2S_LIMIT(C >= 1 && C <= 256, "attention: value width %d outside [1, 256]", C);
     const int dp = d + 1;
     const size_t smem1 = sizeof(float) * ((size_t)TK * dp + TQ * dp + TQ * (TK + 1));
-    F2S_CUDA_TRY(cudaFuncSetAttribute(attn_colstats_kernel,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem1));
+    F2S_TRY(allow_shared(attn_colstats_kernel, smem1));
     const int key_tiles = ceil_div(N, TK);
     {
     TraceScope trace(kTagAttnColstats, stream);

@@ -806,8 +806,7 @@ int attention_tc(const float* q, const float* k, int ldqk, const float* v, int l
         a.tiles = ceil_div(N, kRows);
         a.idesc_s = tc::make_idesc(kRows, kRows, 1u);
         const size_t smem = 1024 + 6 * kRows * 128 + 96 + 2 * kRows * 4 + 32;
-        F2S_CUDA_TRY(cudaFuncSetAttribute(attn_tc_colstats_kernel,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        F2S_TRY(allow_shared(attn_tc_colstats_kernel, smem));
         attn_tc_colstats_kernel<<<B * a.tiles, kThreads, smem, st>>>(map_hi_q, map_lo_q, a);
         F2S_TRY(check_launch("attn_tc_colstats_kernel"));
     }
@@ -825,8 +824,7 @@ int attention_tc(const float* q, const float* k, int ldqk, const float* v, int l
         a.k_stages = smem_for(2) <= 227 * 1024 ? 2 : 1;
         const size_t smem = smem_for(a.k_stages);
         F2S_LIMIT(smem <= 227 * 1024, "attention_tc: %zu bytes of shared memory", smem);
-        F2S_CUDA_TRY(cudaFuncSetAttribute(attn_tc_output_kernel,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        F2S_TRY(allow_shared(attn_tc_output_kernel, smem));
         attn_tc_output_kernel<<<B * a.tiles, kOutThreads, smem, st>>>(
             map_hi_q, map_lo_q, map_hi_k, map_lo_k, map_vt, map_h, map_out, a);
         F2S_TRY(check_launch("attn_tc_output_kernel"));

@@ -23,6 +23,15 @@ inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Number of SMs on the current device (cached per device).
 int sm_count();
 
+// Let `kernel` have `bytes` of dynamic shared memory per block on the current device.
+// The limit belongs to the kernel and is shared by all host threads, so it only grows:
+// lowered for a small call it would refuse the launch of a large one beside it.
+int allow_shared(const void* kernel, size_t bytes);
+template <typename... A>
+int allow_shared(void (*kernel)(A...), size_t bytes) {
+    return allow_shared(reinterpret_cast<const void*>(kernel), bytes);
+}
+
 // Per-launch device timing (CUDA events around each kernel launch), off by
 // default; f2s_trace_enable / f2s_trace_collect expose it through the C-ABI.
 enum TraceTag {

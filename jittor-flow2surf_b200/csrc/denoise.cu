@@ -608,9 +608,7 @@ extern "C" int f2s_fps(const float* points, int64_t N, int64_t count, int64_t fi
         TraceScope trace(kTagFps, st);
         F2S_CUDA_TRY(cudaMemsetAsync(workspace, 0, need, st));
         const size_t smem_bytes = (size_t)grid_slice * 16;
-        F2S_CUDA_TRY(cudaFuncSetAttribute(fps_grid_kernel,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)smem_bytes));
+        F2S_TRY(allow_shared(fps_grid_kernel, smem_bytes));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(grid);
         cfg.blockDim = dim3(kFpsGridThreads);
@@ -646,9 +644,7 @@ extern "C" int f2s_fps(const float* points, int64_t N, int64_t count, int64_t fi
     cfg.numAttrs = 1;
     float* gmin = static_cast<float*>(workspace);
     if (smem) {
-        F2S_CUDA_TRY(cudaFuncSetAttribute(fps_kernel<true>,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)cfg.dynamicSmemBytes));
+        F2S_TRY(allow_shared(fps_kernel<true>, cfg.dynamicSmemBytes));
         F2S_CUDA_TRY(cudaLaunchKernelEx(&cfg, fps_kernel<true>, points, n, (int)count, (int)first,
                                         slice, gmin, selected));
     } else {
@@ -670,8 +666,7 @@ extern "C" int f2s_patch_index(const float* points, int64_t N, const int32_t* se
     int kpow2 = 1;
     while (kpow2 < k) kpow2 <<= 1;
     const size_t smem = (size_t)kpow2 * (sizeof(unsigned long long) + sizeof(int));
-    F2S_CUDA_TRY(cudaFuncSetAttribute(patch_index_kernel,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    F2S_TRY(allow_shared(patch_index_kernel, smem));
     TraceScope trace(kTagPatchIndex, as_stream(stream));
     patch_index_kernel<<<P, kPiThreads, smem, as_stream(stream)>>>(
         points, (int)N, seeds, k, kpow2, beta, neighbors, radial, weights);

@@ -174,8 +174,7 @@ int launch_edge(const EdgeArgs& a, cudaStream_t stream) {
                                          (size_t)kHChunk * (a.cout + 1) + (size_t)ppc * a.cout) +
                         sizeof(int) * kEdgesPerCta;
     auto kernel = edge_kernel<CT>;
-    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)smem));
+    F2S_TRY(allow_shared(kernel, smem));
     const int R = a.B * a.M;
     TraceScope trace(kTagEdge, stream);
     kernel<<<ceil_div(R, ppc), 256, smem, stream>>>(a, ppc);

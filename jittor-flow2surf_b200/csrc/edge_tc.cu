@@ -705,8 +705,7 @@ int edge_stage_tc(const EdgeArgs& e, int precision, cudaStream_t st) {
     const int grid = tiles < sm_count() ? tiles : sm_count();
     TraceScope trace(kTagEdge, st);
     auto launch = [&](auto kernel) -> int {
-        F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)smem));
+        F2S_TRY(allow_shared(kernel, smem));
         kernel<<<grid, kThreads, smem, st>>>(map, a);
         return check_launch("edge_tc_kernel");
     };

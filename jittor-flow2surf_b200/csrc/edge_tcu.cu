@@ -685,8 +685,7 @@ int edge_stage_unified(const EdgeArgs& e, cudaStream_t st) {
     const int grid = tiles < sm_count() ? tiles : sm_count();
     TraceScope trace(kTagEdge, st);
     auto launch = [&](auto kernel) -> int {
-        F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)smem));
+        F2S_TRY(allow_shared(kernel, smem));
         kernel<<<grid, kThreads, smem, st>>>(a);
         return check_launch("edge_unified_kernel");
     };

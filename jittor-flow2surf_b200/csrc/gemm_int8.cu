@@ -290,7 +290,7 @@ int tiles_launch(const Int8Args& a, int split, cudaStream_t st) {
     g.stages = stages;
     const size_t smem = fixed + stages * stage;
     auto kernel = linear_int8_tiles_kernel<T, BN>;
-    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    F2S_TRY(allow_shared(kernel, smem));
     const int token_tiles = ceil_div(a.rows, BN);
     F2S_LIMIT(token_tiles <= 65535, "linear_int8: %d rows", a.rows);
     cudaLaunchConfig_t cfg{};
@@ -754,7 +754,7 @@ int pairs_launch(const Int8Args& a, int bn, cudaStream_t st) {
     g.stages = stages > 8 ? 8 : stages;
     const size_t smem = fixed + g.stages * stage;
     auto kernel = linear_int8_pairs_kernel<T>;
-    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    F2S_TRY(allow_shared(kernel, smem));
     const int tiles = g.m_tiles * g.n_tiles, most = sm_count() / 2, pairs = tiles < most ? tiles : most;
     g.step_bands = pairs / (8 * g.n_tiles);
     g.step_rest = pairs % (8 * g.n_tiles);

@@ -334,7 +334,7 @@ int launch_knn(const float* features, int B, int C, int N, int k, int actual_k, 
     const size_t smem = (size_t)n_pad * 4 + (size_t)kWarps * 256 * 4 + (size_t)kWarps * 64 * 8 + feat;
     auto kernel = knn_kernel<SLOTS, CFIX>;
     if (smem > 48 * 1024)
-        F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        F2S_TRY(f2s::allow_shared(kernel, smem));
     const int tiles = f2s::ceil_div(N, kQueriesPerCta);
     const int64_t grid = (int64_t)B * tiles;
     F2S_LIMIT(grid < (1ll << 31), "knn grid too large: B=%d N=%d", B, N);

@@ -582,8 +582,7 @@ int forward(const Dims& d, const Layout& L, const float* P, const float* x_in, c
         const int grid = blocks < 4 * sm_count() ? blocks : 4 * sm_count();
         auto launch = [&](auto kernel, int S) -> int {
             const size_t smem = sizeof(float) * ((size_t)S * S + 7 * (size_t)S);
-            F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              (int)smem));
+            F2S_TRY(allow_shared(kernel, smem));
             kernel<<<grid, 256, smem, st>>>(x_in, B, M, P + L.in_w, P + L.in_b, P + L.in_ln_w,
                                             P + L.in_ln_b, P + L.in_out_w, P + L.in_out_b, S0,
                                             w.xyz4, w.feat0, nullptr);
@@ -595,8 +594,7 @@ int forward(const Dims& d, const Layout& L, const float* P, const float* x_in, c
     } else {
         const int S0 = d.sd[0];
         const size_t smem = sizeof(float) * ((size_t)S0 * S0 + 8 * S0);
-        F2S_CUDA_TRY(cudaFuncSetAttribute(input_embed_kernel,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        F2S_TRY(allow_shared(input_embed_kernel, smem));
         TraceScope trace(kTagInputEmbed, st);
         const int groups = ceil_div(R, 8);
         const int grid = groups < 4 * sm_count() ? groups : 4 * sm_count();

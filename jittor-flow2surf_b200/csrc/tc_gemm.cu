@@ -805,7 +805,7 @@ int launch_tc(const CUtensorMap& ma, const CUtensorMap& ma2, const CUtensorMap& 
               const CUtensorMap& mb2, const CUtensorMap& my, const TcGemmArgs& g, size_t smem,
               int grid, cudaStream_t st) {
     auto kernel = tc_gemm_kernel<kTf32, kEpi, kSplit, kEW>;
-    F2S_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    F2S_TRY(allow_shared(kernel, smem));
     kernel<<<grid, gemm_threads<kTf32, kSplit, kEW>(), smem, st>>>(ma, ma2, mb, mb2, my, g);
     return check_launch("tc_gemm_kernel");
 }

@@ -225,3 +225,35 @@ def test_linear_int8_from_a_thread_without_a_context(cuda, rows):
     torch.cuda.synchronize()
     assert status[0][0] == f2s._lib.F2S_OK, status
     assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+def test_linear_int8_from_two_host_threads(cuda):
+    """Calls of one kernel with much and little shared memory, from threads that hold
+    no lock of Python's (as a C++ host's): every launch is accepted."""
+    shapes = [(8, 2048, 8192), (8, 130, 128), (8, 2000, 4096), (300, 1024, 1024), (300, 100, 512)]
+    work = []
+    for i, (rows, cols, K) in enumerate(shapes):
+        x, w = eighths(rows, K, i, cuda), eighths(cols, K, i + 10, cuda)
+        y = torch.empty(rows, cols, dtype=torch.bfloat16, device=cuda)
+        args = (x.values.data_ptr(), x.values.stride(0), x.scale.data_ptr(), w.values.data_ptr(), w.values.stride(0),
+                w.scale.data_ptr(), None, y.data_ptr(), cols, 1, rows, cols, K)
+        work.append((f2s.linear_int8(x, w), x, w, y, args, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    entry, refused = f2s._lib.lib().f2s_linear_int8, []
+
+    def calls(args, stream):
+        for _ in range(2000):
+            if entry(*args, stream.cuda_stream) != f2s._lib.F2S_OK:
+                refused.append(f2s._lib.lib().f2s_last_error())
+                return
+
+    threads = [threading.Thread(target=calls, args=item[4:]) for item in work]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert not refused, refused
+    for want, *_, y, _, _ in work:
+        assert torch.equal(y, want)
