@@ -209,8 +209,8 @@ __device__ __forceinline__ float max_abs(const float (&v)[8], float m) {
 template <int TPR>
 __device__ __forceinline__ float lanes_max(float m) {
     if constexpr (TPR >= 32) {
-        float r;
-        asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(m));
+        float r;  // volatile: all 32 lanes execute it, wherever its result is used
+        asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(m));
         return r;
     } else {
 #pragma unroll
