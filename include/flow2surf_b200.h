@@ -232,7 +232,8 @@ int f2s_dequantize_rows(const int8_t* q, int64_t ldq, const float* scale, int64_
  * F2S_ERR_UNSUPPORTED beyond); bias (cols) of dtype or NULL; y of dtype and
  * pitch ldy. On tcgen05 where x and w start on 16 bytes with pitches that are
  * multiples of 16 (as f2s_quantize_rows can lay them out); other pitches run
- * on the CUDA cores.
+ * on the CUDA cores, with at most 4194240 columns. rows and cols at most
+ * 2^31 - 256.
  */
 int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
                     int64_t ldw, const float* w_scale, const void* bias, void* y, int64_t ldy,

@@ -200,7 +200,8 @@ Tensor linear_int8(const Tensor& xv, const Tensor& xs, const Tensor& wv, const T
     Tensor out = at::empty(with_width(xv, cols), xv.options().dtype(type));
     if (out.numel() == 0) return out;
     const Rows x(xv), w(wv);
-    TORCH_CHECK_VALUE(x.rows <= INT32_MAX && cols <= INT32_MAX, "linear_int8 takes at most 2^31 - 1 rows and columns");
+    TORCH_CHECK_VALUE(x.rows <= INT32_MAX - 255 && cols <= INT32_MAX - 255,
+                      "linear_int8 takes at most 2^31 - 256 rows and columns");
     const Tensor xc = xs.contiguous(), wc = ws.contiguous(), b = bias ? bias->contiguous() : Tensor();
     const Launch launch(xv);
     check(f2s_linear_int8(static_cast<const int8_t*>(x.data()), x.pitch, static_cast<const float*>(xc.data_ptr()),

@@ -153,6 +153,9 @@ extern "C" int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scal
     F2S_TRY(f2s::rows::check_dtype("linear_int8", dtype));
     F2S_REQUIRE(rows >= 0 && cols >= 1 && K >= 1, "linear_int8: bad shape rows=%d cols=%d K=%d", rows, cols, K);
     F2S_LIMIT(K <= f2s::kMaxK, "linear_int8: K=%d, at most %d for an exact 32-bit sum", K, f2s::kMaxK);
+    // a tile's last row and column are 32-bit numbers
+    F2S_LIMIT(rows <= INT32_MAX - 255 && cols <= INT32_MAX - 255, "linear_int8: %d x %d outputs, at most 2^31 - 256 a side",
+              rows, cols);
     if (rows == 0) return F2S_OK;
     F2S_REQUIRE(x && x_scale && w && w_scale && y, "linear_int8: null pointer");
     F2S_REQUIRE(ldx >= K && ldw >= K && ldy >= cols, "linear_int8: row pitch below the row");

@@ -135,6 +135,7 @@ extern "C" int f2s_dequantize_rows(const int8_t* q, int64_t ldq, const float* sc
                                    int64_t ldy, int dtype, void* stream) {
     F2S_TRY(f2s::rows::check_dtype("dequantize_rows", dtype));
     F2S_REQUIRE(rows >= 0 && C >= 1, "dequantize_rows: bad shape rows=%lld C=%d", (long long)rows, C);
+    F2S_LIMIT(C <= INT32_MAX - 255, "dequantize_rows: C=%d, at most 2^31 - 256 channels", C);
     if (rows == 0) return F2S_OK;
     F2S_REQUIRE(q && scale && y, "dequantize_rows: null pointer");
     F2S_REQUIRE(ldq >= C && ldy >= C, "dequantize_rows: row pitch below C=%d", C);

@@ -257,3 +257,15 @@ def test_linear_int8_from_two_host_threads(cuda):
     assert not refused, refused
     for want, *_, y, _, _ in work:
         assert torch.equal(y, want)
+
+
+def test_sizes_next_to_31_bits_are_refused():
+    """Tiles end up to 255 rows, columns or channels past a size."""
+    lib, most = f2s._lib.lib(), 2**31 - 256
+    for rows, cols in ((most + 1, 8), (8, most + 1), (2**31 - 1, 8)):
+        assert lib.f2s_linear_int8(16, 16, 16, 16, 16, 16, None, 16, 2**31, 0, rows, cols, 16, None) == f2s._lib.F2S_ERR_UNSUPPORTED
+        assert b"2^31 - 256" in lib.f2s_last_error()
+    assert lib.f2s_dequantize_rows(16, 2**31, 16, 1, most + 1, 16, 2**31, 1, None) == f2s._lib.F2S_ERR_UNSUPPORTED
+    # and what is allowed gets as far as the null pointers
+    assert lib.f2s_linear_int8(None, 16, 16, 16, 16, 16, None, 16, 2**31, 0, most, 8, 16, None) == f2s._lib.F2S_ERR_INVALID_ARGUMENT
+    assert lib.f2s_dequantize_rows(None, 2**31, 16, 1, most, 16, 2**31, 1, None) == f2s._lib.F2S_ERR_INVALID_ARGUMENT
