@@ -5,7 +5,8 @@ Python package (flow2surf_b200/libflow2surf_sm100.so) so that it travels with
 the source tree, and so does the PyTorch binding of the 8-bit feed-forward
 operators (flow2surf_b200/_feedforward.so, from csrc/feedforward_torch.cpp with
 the host compiler). Only sources newer than their object (or than any header)
-are recompiled.
+are recompiled. The library needs nvcc alone; where torch, Python's headers or
+g++ are missing, the binding is left out with a message.
 
     python jittor-flow2surf_b200/build.py [--force] [--jobs N]
 """
@@ -13,6 +14,7 @@ are recompiled.
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -70,6 +72,17 @@ def _compile(src: Path, force: bool, extra: list[str]) -> tuple[Path, str]:
     return obj, proc.stderr
 
 
+def binding_lacks() -> str | None:
+    """What the PyTorch binding cannot be built for, or None."""
+    if importlib.util.find_spec("torch") is None:
+        return "torch is not installed for this interpreter"
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return "Python.h is not installed"
+    if shutil.which("g++") is None:
+        return "g++ not found"
+    return None
+
+
 def _compile_binding(force: bool) -> tuple[Path, str]:
     """Object of the PyTorch binding, against the torch of this interpreter (a
     stamp beside it names their versions)."""
@@ -115,8 +128,9 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     jobs = jobs or min(len(sources), os.cpu_count() or 4)
+    lacks = binding_lacks()
     with ThreadPoolExecutor(max_workers=jobs + 1) as pool:
-        binding = pool.submit(_compile_binding, force)
+        binding = None if lacks else pool.submit(_compile_binding, force)
         results = list(pool.map(lambda s: _compile(s, force, extra or []), sources))
     objects = [obj for obj, _ in results]
     if verbose:
@@ -130,7 +144,11 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
-    _link_binding(binding.result()[0], force)
+    if binding is None:
+        print(f"{BINDING.name} is not built, the 8-bit feed-forward operators have no Python side: {lacks}",
+              file=sys.stderr)
+    else:
+        _link_binding(binding.result()[0], force)
     return LIBRARY
 
 
