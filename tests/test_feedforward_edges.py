@@ -14,8 +14,8 @@ from torch.autograd import forward_ad
 
 import flow2surf_b200 as f2s
 from flow2surf_b200.feedforward import Int8Rows
-from test_feedforward import (DEPTH, NORM, U, close, eighths, half_step, nearest_whole, norm64, norm_grad64, normal,
-                              row_max, smallest)
+from test_feedforward import (DEPTH, NORM, TYPES, U, WIDTHS, close, eighths, half_step, nearest_whole, norm64,
+                              norm_grad64, normal, row_max, smallest)
 
 # fp32 streams and weights s, w of 24 bits with 254 s1 w1 - c s0 w0 = r for c odd:
 # 127 p / m is r / (2 m) off the half c / 2, less than 64-bit products tell (they
@@ -146,6 +146,64 @@ def test_norm_of_rows_whose_reciprocal_leaves_fp32(cuda, sizes, width, dtype):
     close_or_none(got_dx, dx, bound * 1.001 + smallest(dtype))
     terms = (dy.double() * n).abs().sum(0)
     close_or_none(got_dw, dw, half_step(dtype) * dw.abs() + U * (9 + NORM + 1) * terms + smallest(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", WIDTHS)
+def test_norm_int8_of_one_token(cuda, width, dtype):
+    """A decode step's row, as it lies."""
+    x, r = (normal(1, width, dtype=dtype, seed=width + i).to(cuda) for i in (0, 1))
+    w = normal(width, dtype=dtype, seed=2).to(cuda)
+    for added in (r, None):
+        eight, stream = f2s.add_rms_norm_int8(x, w, added)
+        want, s, w64, rstd = norm64(x, w, added, 1e-6)
+        assert torch.equal(stream, want)
+        p = s * w64
+        assert torch.equal(eight.values, nearest_whole(p, row_max(p)))
+        scale = (row_max(p) * rstd / 127)[:, 0]
+        close(eight.scale, scale, scale * (NORM + 2) * U + 1e-45)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_checkpoints_of_every_16_bit_value(cuda, dtype):
+    """Groups that hold all positive values of the binades in which 127 v / m is
+    between 1/4 and 127, for maxima of every kind of significand."""
+    bits = 7 if dtype == torch.bfloat16 else 10
+    significands = torch.arange(2**bits, 2 ** (bits + 1), dtype=torch.float64)
+    values = torch.cat([significands * 2.0**e for e in range(-10, 1)]) * 2.0**-bits  # below 2
+    values = torch.nn.functional.pad(values, (0, -len(values) % 127)).view(-1, 127)
+    maxima = (significands[:: 1 if dtype == torch.bfloat16 else 5] * 2.0**-bits)[:, None, None]
+    held = torch.where(values <= maxima, values, 0.0)
+    held = torch.cat([maxima.expand(-1, len(values), 1), held], 2)  # (maxima, groups, 128)
+    rows, groups = held.shape[:2]
+    want = nearest_whole(held, row_max(held))
+    gate = held.flatten(1)
+    kept, scale = keep_groups(torch.cat([gate, -gate], 1).to(dtype).to(cuda))
+    assert torch.equal(kept[:, :, 0].cpu(), want) and torch.equal(kept[:, :, 1].cpu(), -want)
+    assert torch.equal(scale.cpu(), (maxima / 127).float().expand(rows, groups, 2))
+
+
+def keep_groups(projected):
+    """The forward's checkpoint of whole groups: values (rows, groups, 2, 128) in
+    the channels' order, scales (rows, groups, 2)."""
+    rows, hidden = projected.shape[0], projected.shape[1] // 2
+    groups = hidden // 128
+
+    def call(p):
+        y = p.new_empty(len(p), hidden)
+        kept = torch.empty(len(p), groups, 2, 128, dtype=torch.int8, device=p.device)
+        scale = torch.empty(len(p), groups, 2, device=p.device)
+        f2s._lib.call("f2s_swiglu", p.data_ptr(), 2 * hidden, {torch.bfloat16: 1, torch.float16: 2}[p.dtype], len(p), hidden,
+                      y.data_ptr(), kept.data_ptr(), scale.data_ptr(), f2s._lib.stream_handle())
+        return kept, scale
+
+    # where each channel's byte lies: that of a group whose values name their channels
+    named = torch.arange(128, device=projected.device).repeat(2 * groups).to(projected.dtype)
+    place = call(named[None])[0][0].long().argsort(-1)
+    kept, scale = call(projected)
+    return kept.gather(3, place.expand(rows, -1, -1, -1)), scale
 
 
 def test_forward_mode_derivatives_are_refused():
