@@ -192,7 +192,9 @@ typedef enum f2s_dtype { F2S_DTYPE_F32 = 0, F2S_DTYPE_BF16 = 1, F2S_DTYPE_F16 = 
  * 8-bit rows: q (rows, C) int8 of pitch ldq and one fp32 scale per row, standing
  * for scale * q. q is the whole number nearest to 127 v / max|v| (of the exact
  * quotient, the even one at a tie), scale = max|v| / 127. A row of zeros has
- * scale 0; a row with a value that is not finite has q 0 and scale NaN.
+ * scale 0; a row with a value that is not finite has q 0 and scale NaN (for the
+ * norm's rows: with a product of the stream and the weight that is not, as a real
+ * number; one past fp32 is finite).
  *
  * Root-mean-square norm of a residual stream:
  *   s = x + residual, rounded to dtype and written to stream_out (rows, C);
@@ -227,12 +229,13 @@ int f2s_dequantize_rows(const int8_t* q, int64_t ldq, const float* scale, int64_
                         void* y, int64_t ldy, int dtype, void* stream);
 
 /*
- * y[t, n] = x_scale[t] w_scale[n] sum_k x[t, k] w[n, k] + bias[n]: x (rows, K)
+ * y[t, n] = x_scale[t] w_scale[n] sum_k x[t, k] w[n, k] + bias[n], in fp32 in the
+ * order (sum x_scale) w_scale + bias (a sum x_scale past 3.4e38 is infinite): x (rows, K)
  * and w (cols, K) 8-bit rows, the sum exact in 32 bits (K <= 131071,
  * F2S_ERR_UNSUPPORTED beyond); bias (cols) of dtype or NULL; y of dtype and
  * pitch ldy. On tcgen05 where x and w start on 16 bytes with pitches that are
- * multiples of 16 (as f2s_quantize_rows can lay them out); other pitches run
- * on the CUDA cores, with at most 4194240 columns. rows and cols at most
+ * multiples of 16 (as f2s_quantize_rows can lay them out); other pitches run on
+ * the CUDA cores, 10 to 60 times slower, with at most 4194240 columns. rows and cols at most
  * 2^31 - 256.
  */
 int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
@@ -241,7 +244,7 @@ int f2s_linear_int8(const int8_t* x, int64_t ldx, const float* x_scale, const in
 
 /*
  * SwiGLU of a packed projection (rows, 2 H) = [gate | value]:
- * y = value gate sigma(gate), (rows, H).
+ * y = value gate sigma(gate), (rows, H); sigma below 2^-126 (gates below -87.3) is 0.
  * checkpoint / checkpoint_scale (both or neither): the gate and value rows kept
  * in 8 bits for the backward. With G = ceil(H / F2S_SWIGLU_GROUP) groups of
  * channels a row takes G * 2 * F2S_SWIGLU_GROUP bytes and 2 G scales (gate and

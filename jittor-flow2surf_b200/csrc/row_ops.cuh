@@ -269,8 +269,12 @@ __device__ __forceinline__ void row_sum_max(A& a, M& m, A* shared_a, M* shared_m
 // although exact halves are common then (about one quotient of bf16 values in
 // 1,000, which cost SwiGLU's forward a quarter of its instructions): one step
 // with the exact remainder makes t the rounded quotient itself, exact where that
-// is a half, and every other quotient is 2^-17 from a half or more, the rounding's
-// error 2^-18 or less.
+// is a half, and no other quotient rounds to a half. For v = a u and m = b w, with
+// a and b whole numbers below 2^16 and u and w powers of two, 254 v - c m is a
+// multiple of the smaller of u and w, and the quotient's distance from c / 2 is
+// that over 2 m: where w is the smaller, at least 1 / (2 b) > 2^-17 against a
+// rounding of 2^-18 at most (quotients end at 127); where u is, at least
+// t / (254 a) > 2^-23.99 t against a rounding of 2^-24 t.
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
 constexpr float kBorder = 0.49995f;
 // Below 1e-30, 127 / m may overflow and products lose bits, and above 1e30

@@ -47,8 +47,11 @@ class Int8Rows(NamedTuple):
     """Rows in 8 bits: `values` (..., channels) int8 and `scale` (...) float32,
     standing for values * scale[..., None]. The library's rows start on
     multiples of 16 bytes, which the tensor-core product needs; `values` is
-    then a view of a wider buffer where channels is not a multiple of 16. Scales
-    that want a gradient are refused, since none would come."""
+    then a view of a wider buffer where channels is not a multiple of 16, and
+    clone, to(device), contiguous, cat and indexing give rows without that pitch:
+    linear_int8 takes them too, but on the CUDA cores, 10 to 60 times slower, so
+    move and cut such weights before quantize_rows. Scales that want a gradient
+    are refused, since none would come."""
 
     values: torch.Tensor
     scale: torch.Tensor
@@ -72,8 +75,9 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
     """x weight^T + bias of 8-bit rows x (..., K) and weight (cols, K), with a
     scale per token and per output channel: the sum over K is exact in 32-bit
     integers (K at most 131071), scales and bias (cols, of `dtype`) are applied
-    in fp32, and the result (..., cols) is rounded to `dtype` once. No
-    gradient."""
+    in fp32, the token's scale first (a sum times it beyond 3.4e38 is infinite),
+    and the result (..., cols) is rounded to `dtype` once. Rows and cols at most
+    2^31 - 256. No gradient."""
     xv, xs = x
     wv, ws = weight
     return _native().linear_int8(xv, xs, wv, ws, bias, dtype)
@@ -95,15 +99,17 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
                       *, eps: float = 1e-6) -> tuple[Int8Rows, torch.Tensor]:
     """add_rms_norm with the normed rows in 8 bits, for linear_int8:
     (Int8Rows, stream). The values are the whole numbers nearest to
-    127 p / max|p| with p = stream * weight (the norm cancels), the scale is
-    max|p| / (127 sqrt(mean(stream^2) + eps)). No gradient."""
+    127 p / max|p| with p = stream * weight (the norm cancels, and p may lie past
+    fp32 at either end), the scale is max|p| / (127 sqrt(mean(stream^2) + eps)). No
+    gradient."""
     values, scale, stream = _native().add_rms_norm_int8(x, weight, residual, eps)
     return Int8Rows(values, scale), stream
 
 
 def swiglu(projected: torch.Tensor, *, checkpoint: str | None = None) -> torch.Tensor:
     """value * gate * sigmoid(gate) of a packed projection (..., 2 H) =
-    [gate | value] -> (..., H). Differentiable. `checkpoint` None keeps the
+    [gate | value] -> (..., H). Differentiable. A sigmoid below 2^-126 (gates below
+    -87.3) is 0. `checkpoint` None keeps the
     projection for the backward; "int8" keeps it in 8 bits (a scale for every
     128 channels of the gate and of the value: 52% of the bytes of a 16-bit
     type), and the backward is that of the kept values: each is off by at most

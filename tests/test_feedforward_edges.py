@@ -327,3 +327,21 @@ def test_sizes_next_to_31_bits_are_refused():
     # and what is allowed gets as far as the null pointers
     assert lib.f2s_linear_int8(None, 16, 16, 16, 16, 16, None, 16, 2**31, 0, most, 8, 16, None) == f2s._lib.F2S_ERR_INVALID_ARGUMENT
     assert lib.f2s_dequantize_rows(None, 2**31, 16, 1, most, 16, 2**31, 1, None) == f2s._lib.F2S_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.gpu
+def test_gradients_of_the_two_addends_are_tensors_of_their_own(cuda):
+    """One buffer holds dx for both; what backward() leaves in .grad is not shared."""
+    x, r = (normal(5, 64, seed=s).to(cuda).requires_grad_() for s in (1, 2))
+    w = normal(64, seed=3).to(cuda).requires_grad_()
+    for _ in range(2):  # the second accumulates
+        y, stream = f2s.add_rms_norm(x, w, r)
+        (y.sum() + stream.sum()).backward()
+    assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()
+    held = r.grad.clone()
+    x.grad.zero_()
+    assert torch.equal(r.grad, held)
+    x.grad = r.grad = None
+    f2s.add_rms_norm(x, w, r)[1].sum().backward()  # the stream alone
+    x.grad.zero_()
+    assert (r.grad == 1).all()
